@@ -94,6 +94,7 @@ struct Row {
 
 // Packed fp32 arithmetic for the per-lane row loops (round 4).  At K = 256 the kernel is bound by vector-ALU issue (profiles/r04_cone_pmc.md: ~700 vector
 // instructions per pair, most of them one multiply or one add of a row element); gfx950 issues v_pk_mul_f32 / v_pk_add_f32 on TWO elements at the rate of one.
+// (The build turns packed fp32 instructions OFF -- csrc/Makefile, NOPK -- so today these helpers compile to scalar ones; the pairwise order of the sums stays.)
 // Element arithmetic is unchanged (IEEE multiply and add per element, nothing contracted); a dot product keeps two running sums (even / odd elements) and
 // adds them at the end -- another summation order than the former element-by-element loop, like every order a fixed one against the reference's reduction.
 typedef float f2v __attribute__((ext_vector_type(2)));
