@@ -248,6 +248,41 @@ int lec_multilevel_ce_fwd_bwd(const float* logits, int64_t ld, const int64_t* le
                               lec_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * (6b) Feedback on label paths, beside the multi-level cross-entropy: log-probabilities of paths, preference loss, clipped policy loss.
+ *      No counterpart in the reference (its classifier learns from MultiLevelCELoss alone); the logits and levels are those of loss.py:29-38.
+ *      logits: [R, C] of `dtype` (LEC_DTYPE_*), row stride ld >= C elements, element-aligned; level l owns level_sizes[l] consecutive columns,
+ *      L <= 16, the sizes sum to C.  paths: int64 [R, G, L], G <= 64 paths a row: the class within the level, negative = not counted (its
+ *      logp is 0, its gradient 0, ref / old / coef entries there are not used); a class >= the level's size gives NaN and reads nothing.
+ *      logp / ref / old / coef: fp32 [R, G, L].  Levels that no path of a row counts may hold anything (NaN included): their gradient is 0.
+ *      partials: lec_path_partials_bytes() bytes written by a forward call and read by its backward.  workspace: lec_path_workspace_bytes()
+ *      bytes, written from scratch by every call (nothing has to be cleared, nothing is kept); one call in flight per workspace.
+ *      Every sum has a fixed order: same inputs, same bits.
+ * ------------------------------------------------------------------------------------------------------------- */
+#define LEC_DTYPE_F32   0
+#define LEC_DTYPE_BF16  1
+#define LEC_DTYPE_F16   2
+int64_t lec_path_partials_bytes(int dtype, int64_t R, int C, const int32_t* level_sizes, int L);   /* negative: bad sizes (lec_last_error) */
+int64_t lec_path_workspace_bytes(void);
+int lec_path_logp_fwd(const void* logits, int dtype, int64_t ld, int64_t R, int C, const int32_t* level_sizes, int L, const int64_t* paths, int G,
+                      float* logp, void* partials, lec_stream_t stream);
+/* d logits [R, C] (ldg, of `dtype`) of sum(coef * logp) * up[0] * norm[0]; up, norm: device scalars or NULL.  The backward of all three. */
+int lec_path_logp_bwd(const void* logits, int dtype, int64_t ld, int64_t R, int C, const int32_t* level_sizes, int L, const int64_t* paths, int G,
+                      const void* partials, const float* coef, const float* up, const float* norm, void* dlogits, int64_t ldg, lec_stream_t stream);
+/* P pairs (chosen, rejected).  shared: logits [P, C], paths [P, 2, L]; else logits [2P, C], paths [2P, L], the P chosen first.
+ *   reward = beta * sum_l (logp - ref);  d = reward_chosen - reward_rejected
+ *   loss[0] = mean (1 - s) softplus(-d) + s softplus(d), s = label_smoothing;  rewards: fp32 [P, 2];  coef = d loss / d logp, as paths. */
+int lec_preference_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t P, int shared, int C, const int32_t* level_sizes, int L, const int64_t* paths,
+                            const float* ref, float beta, float label_smoothing, float* loss, float* rewards, float* coef, void* partials, void* workspace,
+                            int64_t workspace_bytes, lec_stream_t stream);
+/* rho = exp(logp - old) (old_logp NULL: 1), A = adv[r, g], q = ref - logp (ref_logp NULL: no KL term, kl_coef must be 0)
+ *   t = -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1)
+ *   loss[0] = mean of t;  stats[0] = mean of (exp(q) - q - 1), stats[1] = clipped share;  norm[0] = a factor of the gradient (lec_path_logp_bwd's norm)
+ *   mean: per_path == 0: over the counted entries (0 when there are none); else over all R G paths of each path's mean over its counted entries. */
+int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t R, int C, const int32_t* level_sizes, int L, const int64_t* paths, int G, const float* adv,
+                        const float* old_logp, const float* ref_logp, float clip_low, float clip_high, float kl_coef, int per_path, float* loss, float* stats,
+                        float* norm, float* coef, void* partials, void* workspace, int64_t workspace_bytes, lec_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * (7) Fused BatchNorm (+ residual add) (+ ReLU) on NHWC bf16 activations -- the HBM-bound half of the ResNet backbone
  *     behind FeatCNN18 / FeatCNN (oe_h.py:311,317 -> torchvision BasicBlock/Bottleneck: `relu(bn(conv(x)))`,
  *     `relu(bn(conv(x)) + identity)`, downsample `bn(conv(x))`) and their autograd.

@@ -5,12 +5,13 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('LEC_LIB_PATH') or os.path.join(_HERE, 'liblecone.so')     # LEC_LIB_PATH: A/B builds of the same ABI
-ABI_VERSION = 33
+ABI_VERSION = 34
 
 OK, E_ARG, E_HIP, E_EMPTY, E_STATE = 0, -1, -2, -3, -4
 ENERGY_HYP_CONE, ENERGY_ORDER, ENERGY_EUC_CONE = 0, 1, 2
 LABEL_RAW, LABEL_HYP, LABEL_SOFTCLIP_K = 0, 1, 2
 IMAGE_RAW, IMAGE_SOFTCLIP, IMAGE_SOFTCLIP_K = 0, 1, 2
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 SCHEDULE_DEFAULT, SCHEDULE_TILE_WALK, SCHEDULE_AUTO, SCHEDULE_BALANCED = -1, 0, 1, 2
 
 
@@ -74,6 +75,12 @@ def _load():
         'lec_dp_allreduce_sum': (i32, [p, p, i64, i32, p]),
         'lec_dp_destroy': (None, [p]),
         'lec_multilevel_ce_fwd_bwd': (i32, [p, i64, p, i32, i32, p, p, p, i32, p, p, p, i64, p]),
+        'lec_path_partials_bytes': (i64, [i32, i64, i32, p, i32]),
+        'lec_path_workspace_bytes': (i64, []),
+        'lec_path_logp_fwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p]),
+        'lec_path_logp_bwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p, p, p, i64, p]),
+        'lec_preference_loss_fwd': (i32, [p, i32, i64, i64, i32, i32, p, i32, p, p, f32, f32, p, p, p, p, p, i64, p]),
+        'lec_policy_loss_fwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p, f32, f32, f32, i32, p, p, p, p, p, p, i64, p]),
         'lec_bn_workspace_bytes': (i64, [i32]),
         'lec_bn_fwd': (i32, [p, p, i64, i32, p, p, f32, f32, p, p, i32, p, p, p, i32, p, p, i64, p]),
         'lec_bn_bwd': (i32, [p, p, p, p, p, i64, i32, p, p, p, p, p, p, p, i32, p, i64, i32, p]),

@@ -1,0 +1,510 @@
+// Learning from feedback on label paths: log-probabilities of paths, the preference loss and the clipped policy loss, forward and backward.
+//
+// A classifier's logits row z [C] is cut into L levels (network/loss.py:29-38 slices it the same way); each level has a softmax of its own.  A PATH is one class
+// per level, -1 where it is not known; G paths may share a row (two answers of an annotator, the samples of a policy).
+//   lse_l       = m_l + log sum_i exp(z_i - m_l)                       i over level l
+//   logp[r,g,l] = z[r, start_l + y] - lse_l                             (0 where y < 0; NaN where y is no class of the level: nothing is read there)
+//   dz[r,i]     = sum_g c[r,g,l] [y_g = i]  -  (sum_g c[r,g,l]) softmax_l(z)_i       c = d loss / d logp
+// Both losses are functions of logp, so one pair of passes over the logits serves all three: `path_stats` (read z once) and `path_grad` (read z, write dz); between
+// them a small kernel per loss works on [R, G, L] numbers in 64 bits and leaves c.
+//
+// What bounds it: HBM, and at the small sizes the launches (2 forward, 1 backward).  A WAVE owns a run of at most 64 * NL 16-byte vectors of one level of one row,
+// all loaded before the first use, so a level of 39 078 classes spreads over 16 waves and a row of 723 over 4, with no barrier and no LDS; (max, sum) of each run
+// goes to `partials`, and whoever needs a level's lse merges its few runs again in the same order (the saved state of the backward pass IS `partials`).
+// Vectors start at the level's first class, which no alignment is promised for: the loads are 16 bytes wide at element alignment.
+#include "lec_common.h"
+#include <hip/hip_fp16.h>
+#include <hip/hip_bf16.h>
+
+namespace lec {
+
+constexpr int kMaxLevels = 16;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct PathTable {
+  int L, S, G;
+  int start[kMaxLevels + 1];     // first class of a level
+  int first[kMaxLevels + 1];     // first run of a level
+  int vpr[kMaxLevels];           // 16-byte vectors of a run
+};
+
+template <typename T> struct Elt;
+template <> struct Elt<float> {
+  static constexpr int V = 4, NL = 9;
+  static __device__ __forceinline__ float get(const uint4& w, int e) { return __uint_as_float(e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w); }
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[4]) { return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])); }
+  static __device__ __forceinline__ float cvt(float f) { return f; }
+};
+__device__ __forceinline__ unsigned int word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+template <> struct Elt<__hip_bfloat16> {
+  static constexpr int V = 8, NL = 5;
+  static __device__ __forceinline__ float get(const uint4& w, int e) { const unsigned int u = word_of(w, e >> 1); return __uint_as_float((e & 1) ? (u & 0xffff0000u) : (u << 16)); }
+  static __device__ __forceinline__ float load(const __hip_bfloat16* p) { return __uint_as_float((unsigned int)*(const unsigned short*)p << 16); }
+  static __device__ __forceinline__ __hip_bfloat16 cvt(float f) { return __float2bfloat16(f); }        // nearest, ties to even; NaN stays NaN
+  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+    unsigned int u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __hip_bfloat16 a = cvt(f[2 * i]), b = cvt(f[2 * i + 1]);
+      u[i] = (unsigned int)*(const unsigned short*)&a | ((unsigned int)*(const unsigned short*)&b << 16);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+template <> struct Elt<_Float16> {
+  static constexpr int V = 8, NL = 5;
+  static __device__ __forceinline__ float get(const uint4& w, int e) {
+    const unsigned int u = word_of(w, e >> 1);
+    const unsigned short h = (unsigned short)((e & 1) ? (u >> 16) : (u & 0xffffu));
+    return (float)__builtin_bit_cast(_Float16, h);
+  }
+  static __device__ __forceinline__ float load(const _Float16* p) { return (float)*p; }
+  static __device__ __forceinline__ _Float16 cvt(float f) { return (_Float16)f; }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+    unsigned int u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      u[i] = (unsigned int)__builtin_bit_cast(unsigned short, cvt(f[2 * i])) | ((unsigned int)__builtin_bit_cast(unsigned short, cvt(f[2 * i + 1])) << 16);
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+
+// 16 bytes at element alignment (the compiler emits one dwordx4 access: the target's unaligned access mode)
+template <typename T> __device__ __forceinline__ uint4 load16(const T* p) { uint4 w; __builtin_memcpy(&w, (const void*)p, 16); return w; }
+template <typename T> __device__ __forceinline__ void store16(T* p, const uint4& w) { __builtin_memcpy((void*)p, &w, 16); }
+
+__device__ __forceinline__ float fast_exp(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }      // t <= 0: absolute error of a softmax term below 2^-23
+
+// One run: elements [lo, hi) of the level, lane-strided vectors.  x[j][e] = -inf outside.
+template <typename T>
+struct Run {
+  static constexpr int V = Elt<T>::V, NL = Elt<T>::NL;
+  float x[NL][V];
+  __device__ __forceinline__ void load(const T* z, int v0, int nv, int n, int lane) {     // vectors v0 .. v0 + nv of a level of n elements at z
+    uint4 w[NL];
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int k = j * 64 + lane, e0 = (v0 + k) * V;
+      if (k < nv && e0 + V <= n) w[j] = load16(z + e0);
+    }
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int k = j * 64 + lane, e0 = (v0 + k) * V;
+      const bool full = k < nv && e0 + V <= n;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[j][e] = full ? Elt<T>::get(w[j], e) : -INFINITY;
+      if (k < nv && !full) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) if (e0 + e < n) x[j][e] = Elt<T>::load(z + e0 + e);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ int level_of(const PathTable& t, int slot) {
+  int l = 0;
+  while (l + 1 < t.L && slot >= t.first[l + 1]) ++l;
+  return l;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z, int64_t ld, int64_t R, PathTable t, float2* __restrict__ partials, unsigned int* counter) {
+  const int lane = threadIdx.x & 63;
+  if (counter && blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;              // armed for the loss kernel behind this launch
+  const int64_t ntask = R * t.S, nwave = (int64_t)gridDim.x * 4;
+  for (int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); task < ntask; task += nwave) {
+    const int64_t r = task / t.S;
+    const int slot = (int)(task - r * t.S), l = level_of(t, slot), n = t.start[l + 1] - t.start[l];
+    constexpr int V = Elt<T>::V, NL = Elt<T>::NL;
+    const int v0 = (slot - t.first[l]) * t.vpr[l], nv = min(t.vpr[l], (n + V - 1) / V - v0);
+    Run<T> run;
+    run.load(z + r * ld + t.start[l], v0, nv, n, lane);
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NL; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) m = fmaxf(m, run.x[j][e]);
+    m = group_max<64>(m);
+    const float mm = m == -INFINITY ? 0.0f : m;                                  // nothing finite: the terms are exp(-inf) = 0 (NaN stays NaN)
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NL; ++j)
+      if (j * 64 < nv) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += fast_exp(run.x[j][e] - mm);
+      }
+    s = group_sum<64>(s);
+    if (lane == 0) partials[task] = make_float2(m, s);
+  }
+}
+
+// (max, sum) of a whole level from its runs, in the order of the runs
+__device__ __forceinline__ float2 merge_runs(const float2* __restrict__ p, int n) {
+  float m = -INFINITY;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, p[i].x);
+  float s = 0.0f;
+  for (int i = 0; i < n; ++i) {
+    const float2 q = p[i];
+    s += q.x == m ? q.y : q.y * fast_exp(q.x - m);                               // (q.x = -inf beside a finite m: 0 * exp(-inf) = 0)
+  }
+  return make_float2(m, s);
+}
+
+// log-probability of class y of level l of row r in 64 bits: (z - m) - log s
+template <typename T>
+__device__ __forceinline__ double entry_logp(const T* __restrict__ z, int64_t ld, int64_t r, const PathTable& t, int l, int64_t y, const float2* __restrict__ partials) {
+  const int n = t.start[l + 1] - t.start[l];
+  if (y >= n) return __builtin_nan("");
+  const float zy = Elt<T>::load(z + r * ld + t.start[l] + y);
+  const float2 ms = merge_runs(partials + r * t.S + t.first[l], t.first[l + 1] - t.first[l]);
+  return ((double)zy - (double)ms.x) - log((double)ms.y);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void path_logp_kernel(const T* __restrict__ z, int64_t ld, int64_t n_entries, PathTable t, const int64_t* __restrict__ paths,
+                                                        const float2* __restrict__ partials, float* __restrict__ logp) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n_entries; i += (int64_t)gridDim.x * 256) {
+    const int l = (int)(i % t.L);
+    const int64_t r = i / ((int64_t)t.L * t.G), y = paths[i];
+    logp[i] = y < 0 ? 0.0f : (float)entry_logp(z, ld, r, t, l, y, partials);
+  }
+}
+
+// Sum of N doubles over the grid in a fixed order; true in thread 0 of the last block, `total` valid there.  Same hand-off as block_publish_and_finalize
+// (lec_common.h); `counter` was zeroed by the launch before.  All threads of the block call it (256 threads).
+template <int N>
+__device__ __forceinline__ bool grid_sum(double (&v)[N] /* one value a thread */, double* __restrict__ block_sums, unsigned int* counter, double (&total)[N]) {
+  __shared__ double s_w[4][N];
+  __shared__ int s_last;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    for (int m = 32; m >= 1; m >>= 1) v[k] += __shfl_xor(v[k], m, 64);
+    if (lane == 0) s_w[w][k] = v[k];
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) block_sums[(int64_t)blockIdx.x * N + k] = s_w[0][k] + s_w[1][k] + s_w[2][k] + s_w[3][k];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const unsigned int prev = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = prev == gridDim.x - 1;
+    if (s_last) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+  }
+  __syncthreads();
+  if (!s_last || w != 0) return false;
+#pragma unroll
+  for (int k = 0; k < N; ++k) total[k] = 0.0;
+  for (unsigned int i = lane; i < gridDim.x; i += 64)
+#pragma unroll
+    for (int k = 0; k < N; ++k) total[k] += block_sums[(int64_t)i * N + k];
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    for (int m = 32; m >= 1; m >>= 1) total[k] += __shfl_xor(total[k], m, 64);
+  return lane == 0;
+}
+
+// Preference loss.  Pair p: reward of a side = beta * sum_l (logp - ref), d = chosen - rejected,
+//   loss = mean_p (1 - eps) softplus(-d) + eps softplus(d) ;  d loss / d d = (eps sigma(d) - (1 - eps) sigma(-d)) / P .
+// 16 lanes a side (one a level), 32 a pair.  shared: both paths score row p; otherwise rows p and P + p.
+template <typename T>
+__global__ __launch_bounds__(256) void preference_kernel(const T* __restrict__ z, int64_t ld, int64_t P, int shared, PathTable t, const int64_t* __restrict__ paths,
+                                                         const float* __restrict__ ref, float beta, float eps, const float2* __restrict__ partials, float* __restrict__ coef,
+                                                         float* __restrict__ rewards, float* __restrict__ loss, double* __restrict__ block_sums, unsigned int* counter) {
+  const int l = threadIdx.x & 15, side = (threadIdx.x >> 4) & 1;
+  double acc[1] = {0.0};
+  // every lane of a wave takes part in the shuffles: the loop bound is the block's, a lane past the last pair works on nothing
+  for (int64_t p0 = (int64_t)blockIdx.x * 8; p0 < P; p0 += (int64_t)gridDim.x * 8) {
+    const int64_t p = p0 + (threadIdx.x >> 5);
+    const bool in = p < P && l < t.L;
+    const int64_t row = shared ? p : side * P + p, entry = ((shared ? p * 2 + side : row)) * t.L + l;
+    const int64_t y = in ? paths[entry] : -1;
+    double r = 0.0;
+    if (y >= 0) r = entry_logp(z, ld, row, t, l, y, partials) - (double)ref[entry];
+    for (int m = 8; m >= 1; m >>= 1) r += __shfl_xor(r, m, 16);
+    r *= (double)beta;
+    const double other = __shfl_xor(r, 16, 32), d = side ? other - r : r - other;
+    const double e = exp(-fabs(d)), lp = log1p(e);                               // softplus(-d) = max(-d, 0) + log1p(exp(-|d|))
+    const double sp = 1.0 / (1.0 + e), sm = e / (1.0 + e);                       // sigma(|d|), sigma(-|d|)
+    const double sig = d >= 0.0 ? sp : (d < 0.0 ? sm : d), sigm = d >= 0.0 ? sm : (d < 0.0 ? sp : d);      // (NaN stays NaN)
+    if (p < P && l == 0) rewards[p * 2 + side] = (float)r;
+    if (p < P && l == 0 && side == 0)
+      acc[0] += (1.0 - (double)eps) * ((d < 0.0 ? -d : d > 0.0 ? 0.0 : d * 0.0) + lp) + (eps != 0.0f ? (double)eps * ((d > 0.0 ? d : d < 0.0 ? 0.0 : d * 0.0) + lp) : 0.0);
+    if (in) {
+      const double g = ((double)eps * sig - (1.0 - (double)eps) * sigm) * (double)beta / (double)P;
+      coef[entry] = y >= 0 ? (float)(side ? -g : g) : 0.0f;
+    }
+  }
+  double total[1];
+  if (grid_sum<1>(acc, block_sums, counter, total)) loss[0] = (float)(total[0] / (double)P);
+}
+
+// Clipped policy loss.  Entry (r, g, l) counted: rho = exp(logp - old), A = advantage[r, g],
+//   t = -min(rho A, clip(rho, 1 - lo, 1 + hi) A) + kl (exp(q) - q - 1),  q = ref - logp ;  dt/dlogp = -rho A [inside or on the bound] - kl expm1(q)
+// loss = sum w t.  mean over counted entries: w = 1 / N, N known only at the end of this launch -- c is left without it and `norm` = 1 / max(N, 1) multiplies it in
+// the backward pass; mean over paths: w = 1 / (entries of the path) / (R G), norm = 1.  stats = {sum w k3, sum w [clipped]}.
+// A path is LW = the power of two >= L lanes of a wave.
+template <typename T>
+__global__ __launch_bounds__(256) void policy_kernel(const T* __restrict__ z, int64_t ld, int64_t n_paths, int LW, PathTable t, const int64_t* __restrict__ paths,
+                                                     const float* __restrict__ adv, const float* __restrict__ old, const float* __restrict__ ref, float lo, float hi, float kl,
+                                                     int per_path, const float2* __restrict__ partials, float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ stats, float* __restrict__ norm,
+                                                     double* __restrict__ block_sums, unsigned int* counter) {
+  const int l = threadIdx.x & (LW - 1), per_block = 256 / LW;
+  const int sh = 31 - __builtin_clz(LW);
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int64_t q0 = (int64_t)blockIdx.x * per_block; q0 < n_paths; q0 += (int64_t)gridDim.x * per_block) {
+    const int64_t q = q0 + (threadIdx.x >> sh);
+    const bool in = q < n_paths && l < t.L;
+    const int64_t entry = q * t.L + l, y = in ? paths[entry] : -1, row = q / t.G;
+    const bool on = y >= 0;
+    const unsigned long long mask = __ballot(on) >> ((threadIdx.x & 63) & ~(LW - 1));
+    const int cnt = __popcll(mask & ((1ull << LW) - 1ull));
+    float c = 0.0f;
+    if (on) {
+      const double lp = entry_logp(z, ld, row, t, l, y, partials), A = (double)adv[q];
+      const double rho = old ? exp(lp - (double)old[entry]) : exp(lp - lp);       // (no old log-probabilities: on-policy, the ratio is 1)
+      const bool clipped = (A > 0.0 && rho > 1.0 + (double)hi) || (A < 0.0 && rho < 1.0 - (double)lo);
+      const double gain = clipped ? (A > 0.0 ? 1.0 + (double)hi : 1.0 - (double)lo) * A : rho * A;
+      double k3 = 0.0, dk = 0.0;
+      if (ref) { const double d = (double)ref[entry] - lp, em = expm1(d); k3 = em - d; dk = em; }
+      const double w = per_path ? 1.0 / ((double)cnt * (double)n_paths) : 1.0;
+      acc[0] += w * ((kl != 0.0f ? (double)kl * k3 : 0.0) - gain);
+      acc[1] += w * k3;
+      acc[2] += clipped ? w : 0.0;
+      acc[3] += 1.0;
+      c = (float)(w * ((clipped ? 0.0 : -rho * A) - (kl != 0.0f ? (double)kl * dk : 0.0)));
+    }
+    if (in) coef[entry] = c;
+  }
+  double total[4];
+  if (grid_sum<4>(acc, block_sums, counter, total)) {
+    const double inv = per_path ? 1.0 : 1.0 / (total[3] > 1.0 ? total[3] : 1.0);
+    loss[0] = (float)(total[0] * inv); stats[0] = (float)(total[1] * inv); stats[1] = (float)(total[2] * inv); norm[0] = (float)inv;
+  }
+}
+
+// dz of one run.  Lane g holds path g of the row (G <= 64): its class y, its coefficient c.  A = sum of the counted c; the softmax part is -A exp(z - m) / s.
+// A == 0 (nothing counted, everything clipped, or the two sides of a preference on one row, whose coefficients are opposite): the part is zero and z is not read.
+// The classes the paths name are written again, by the first lane that names them, with every path's coefficient added in lane order -- after the wave's own
+// vector stores have been acknowledged (one wave writes the whole run, so no other wave is involved).
+template <typename T>
+__global__ __launch_bounds__(256) void path_grad_kernel(const T* __restrict__ z, int64_t ld, int64_t R, PathTable t, const int64_t* __restrict__ paths,
+                                                        const float2* __restrict__ partials, const float* __restrict__ coef, const float* __restrict__ up,
+                                                        const float* __restrict__ norm, T* __restrict__ dz, int64_t ldg) {
+  const int lane = threadIdx.x & 63;
+  const int64_t ntask = R * t.S, nwave = (int64_t)gridDim.x * 4;
+  const float scale = (up ? *up : 1.0f) * (norm ? *norm : 1.0f);
+  for (int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); task < ntask; task += nwave) {
+    constexpr int V = Elt<T>::V, NL = Elt<T>::NL;
+    const int64_t r = task / t.S;
+    const int slot = (int)(task - r * t.S), l = level_of(t, slot), n = t.start[l + 1] - t.start[l];
+    const int v0 = (slot - t.first[l]) * t.vpr[l], nv = min(t.vpr[l], (n + V - 1) / V - v0);
+    const T* zl = z + r * ld + t.start[l];
+    T* gl = dz + r * ldg + t.start[l];
+    int64_t y = -1;
+    float c = 0.0f;
+    if (lane < t.G) {
+      const int64_t e = (r * t.G + lane) * t.L + l;
+      y = paths[e];
+      if (y < 0) y = -1;
+      else c = coef[e] * scale;
+      if (y >= n) c = __builtin_nanf("");
+    }
+    const float A = group_sum<64>(c);
+    float k = 0.0f, m = 0.0f;
+    Run<T> run;
+    if (A != 0.0f) {                                                              // (true for NaN)
+      run.load(zl, v0, nv, n, lane);
+      const float2 ms = merge_runs(partials + r * t.S + t.first[l], t.first[l + 1] - t.first[l]);
+      m = ms.x; k = -A / ms.y;
+#pragma unroll
+      for (int j = 0; j < NL; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) run.x[j][e] = k * fast_exp(run.x[j][e] - m);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NL; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) run.x[j][e] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int i = j * 64 + lane, e0 = (v0 + i) * V;
+      if (i < nv) {
+        if (e0 + V <= n) store16(gl + e0, Elt<T>::pack(run.x[j]));
+        else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) if (e0 + e < n) gl[e0 + e] = Elt<T>::cvt(run.x[j][e]);
+        }
+      }
+    }
+    const bool mine = y >= (int64_t)v0 * V && y < (int64_t)(v0 + nv) * V && y < n;
+    if (__ballot(mine)) {
+      float tot = 0.0f;
+      bool leader = mine;
+      for (int g = 0; g < t.G; ++g) {
+        const int yg = __builtin_amdgcn_readlane((int)(y > n ? n : y), g);
+        const float cg = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), g));
+        if (yg == (int)y) { tot += cg; if (g < lane) leader = false; }
+      }
+      float soft = 0.0f;
+      if (leader && A != 0.0f) soft = k * fast_exp(Elt<T>::load(zl + y) - m);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                            // the vector stores above are in the cache before the same bytes are written again
+      if (leader) gl[y] = Elt<T>::cvt(tot + soft);
+    }
+  }
+}
+
+static int build_table(PathTable& t, const int32_t* sizes, int L, int C, int G, int V, int NL) {
+  t.L = L; t.G = G; t.start[0] = 0; t.first[0] = 0;
+  int64_t s = 0;
+  for (int l = 0; l < L; ++l) {
+    if (sizes[l] <= 0) { set_error("path loss: empty level %d", l); return LEC_E_ARG; }
+    s += sizes[l];
+    if (s > C) break;
+    const int64_t nvec = ((int64_t)sizes[l] + V - 1) / V, cap = (int64_t)64 * NL, np = (nvec + cap - 1) / cap;
+    t.vpr[l] = (int)((nvec + np - 1) / np);
+    t.start[l + 1] = (int)s;
+    t.first[l + 1] = t.first[l] + (int)((nvec + t.vpr[l] - 1) / t.vpr[l]);
+  }
+  if (s != C) { set_error("path loss: level sizes sum to %lld or more, expected C=%d", (long long)s, C); return LEC_E_ARG; }
+  t.S = t.first[L];
+  return LEC_OK;
+}
+
+static int64_t wave_grid(int64_t waves) { const int64_t b = (waves + 3) / 4; return b > (1 << 22) ? (1 << 22) : b; }
+constexpr int64_t kMaxSumBlocks = 2048;
+
+// workspace: [0, 256) the arrival counter | block sums (2048 x 4 doubles)
+constexpr int64_t kWorkBytes = 256 + kMaxSumBlocks * 4 * 8;
+
+template <typename F> static int by_type(int dtype, F&& f) {
+  switch (dtype) {
+    case LEC_DTYPE_F32: f((const float*)nullptr); return LEC_OK;
+    case LEC_DTYPE_BF16: f((const __hip_bfloat16*)nullptr); return LEC_OK;
+    case LEC_DTYPE_F16: f((const _Float16*)nullptr); return LEC_OK;
+  }
+  set_error("path loss: unknown dtype %d", dtype);
+  return LEC_E_ARG;
+}
+
+static int table_for(PathTable& t, int dtype, int64_t R, int C, const int32_t* sizes, int L, int G) {
+  LEC_CHECK_ARG(dtype == LEC_DTYPE_F32 || dtype == LEC_DTYPE_BF16 || dtype == LEC_DTYPE_F16, "path loss: unknown dtype %d", dtype);
+  LEC_CHECK_ARG(sizes && L > 0 && L <= kMaxLevels && C > 0, "path loss: bad levels L=%d (1..%d) C=%d", L, kMaxLevels, C);
+  LEC_CHECK_ARG(R >= 0 && R <= (int64_t)1 << 31 && G > 0 && G <= 64, "path loss: bad sizes rows=%lld paths per row=%d (1..64)", (long long)R, G);
+  return dtype == LEC_DTYPE_F32 ? build_table(t, sizes, L, C, G, Elt<float>::V, Elt<float>::NL) : build_table(t, sizes, L, C, G, Elt<_Float16>::V, Elt<_Float16>::NL);
+}
+
+static int run_stats(const void* z, int dtype, int64_t ld, int64_t R, const PathTable& t, float2* partials, unsigned int* counter, hipStream_t st) {
+  const int rc = by_type(dtype, [&](auto* tag) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
+    hipLaunchKernelGGL((path_stats_kernel<T>), dim3((unsigned)wave_grid(R * t.S)), dim3(256), 0, st, (const T*)z, ld, R, t, partials, counter);
+  });
+  if (rc != LEC_OK) return rc;
+  LEC_CHECK_LAUNCH("path_stats_kernel");
+  return LEC_OK;
+}
+
+}  // namespace lec
+
+extern "C" int64_t lec_path_partials_bytes(int dtype, int64_t R, int C, const int32_t* level_sizes, int L) {
+  using namespace lec;
+  PathTable t;
+  const int rc = table_for(t, dtype, R, C, level_sizes, L, 1);
+  return rc != LEC_OK ? rc : R * t.S * (int64_t)sizeof(float2);
+}
+
+extern "C" int64_t lec_path_workspace_bytes(void) { return lec::kWorkBytes; }
+
+extern "C" int lec_path_logp_fwd(const void* logits, int dtype, int64_t ld, int64_t R, int C, const int32_t* level_sizes, int L, const int64_t* paths, int G,
+                                 float* logp, void* partials, lec_stream_t stream) {
+  using namespace lec;
+  PathTable t;
+  const int rc = table_for(t, dtype, R, C, level_sizes, L, G);
+  if (rc != LEC_OK) return rc;
+  LEC_CHECK_ARG(R > 0 && logits && paths && logp && partials && ld >= C, "path_logp_fwd: null pointer or ld=%lld < C=%d or no rows", (long long)ld, C);
+  hipStream_t st = (hipStream_t)stream;
+  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, nullptr, st);
+  if (rs != LEC_OK) return rs;
+  const int64_t n = R * G * L, blocks = (n + 255) / 256;
+  by_type(dtype, [&](auto* tag) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
+    hipLaunchKernelGGL((path_logp_kernel<T>), dim3((unsigned)(blocks > (1 << 20) ? (1 << 20) : blocks)), dim3(256), 0, st, (const T*)logits, ld, n, t, paths, (const float2*)partials, logp);
+  });
+  LEC_CHECK_LAUNCH("path_logp_kernel");
+  return LEC_OK;
+}
+
+extern "C" int lec_path_logp_bwd(const void* logits, int dtype, int64_t ld, int64_t R, int C, const int32_t* level_sizes, int L, const int64_t* paths, int G,
+                                 const void* partials, const float* coef, const float* up, const float* norm, void* dlogits, int64_t ldg, lec_stream_t stream) {
+  using namespace lec;
+  PathTable t;
+  const int rc = table_for(t, dtype, R, C, level_sizes, L, G);
+  if (rc != LEC_OK) return rc;
+  LEC_CHECK_ARG(R > 0 && logits && paths && partials && coef && dlogits && ld >= C && ldg >= C, "path_logp_bwd: null pointer or ld < C or no rows");
+  by_type(dtype, [&](auto* tag) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
+    hipLaunchKernelGGL((path_grad_kernel<T>), dim3((unsigned)wave_grid(R * t.S)), dim3(256), 0, (hipStream_t)stream, (const T*)logits, ld, R, t, paths,
+                       (const float2*)partials, coef, up, norm, (T*)dlogits, ldg);
+  });
+  LEC_CHECK_LAUNCH("path_grad_kernel");
+  return LEC_OK;
+}
+
+extern "C" int lec_preference_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t P, int shared, int C, const int32_t* level_sizes, int L, const int64_t* paths,
+                                       const float* ref, float beta, float label_smoothing, float* loss, float* rewards, float* coef, void* partials, void* workspace,
+                                       int64_t workspace_bytes, lec_stream_t stream) {
+  using namespace lec;
+  PathTable t;
+  const int64_t R = shared ? P : 2 * P;
+  const int rc = table_for(t, dtype, R, C, level_sizes, L, shared ? 2 : 1);
+  if (rc != LEC_OK) return rc;
+  LEC_CHECK_ARG(P > 0 && logits && paths && ref && loss && rewards && coef && partials && ld >= C, "preference_loss: null pointer or ld=%lld < C=%d or no pairs", (long long)ld, C);
+  LEC_CHECK_ARG(workspace && workspace_bytes >= kWorkBytes, "preference_loss: workspace needs %lld bytes", (long long)kWorkBytes);
+  LEC_CHECK_ARG(label_smoothing >= 0.0f && label_smoothing <= 1.0f, "preference_loss: label_smoothing %g is not in [0, 1]", (double)label_smoothing);
+  hipStream_t st = (hipStream_t)stream;
+  unsigned int* counter = (unsigned int*)workspace;
+  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, counter, st);
+  if (rs != LEC_OK) return rs;
+  const int64_t blocks = (P + 7) / 8;
+  by_type(dtype, [&](auto* tag) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
+    hipLaunchKernelGGL((preference_kernel<T>), dim3((unsigned)(blocks > kMaxSumBlocks ? kMaxSumBlocks : blocks)), dim3(256), 0, st, (const T*)logits, ld, P, shared, t, paths, ref,
+                       beta, label_smoothing, (const float2*)partials, coef, rewards, loss, (double*)((char*)workspace + 256), counter);
+  });
+  LEC_CHECK_LAUNCH("preference_kernel");
+  return LEC_OK;
+}
+
+extern "C" int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t R, int C, const int32_t* level_sizes, int L, const int64_t* paths, int G, const float* adv,
+                                   const float* old_logp, const float* ref_logp, float clip_low, float clip_high, float kl_coef, int per_path, float* loss, float* stats, float* norm, float* coef,
+                                   void* partials, void* workspace, int64_t workspace_bytes, lec_stream_t stream) {
+  using namespace lec;
+  PathTable t;
+  const int rc = table_for(t, dtype, R, C, level_sizes, L, G);
+  if (rc != LEC_OK) return rc;
+  LEC_CHECK_ARG(R > 0 && logits && paths && adv && loss && stats && norm && coef && partials && ld >= C, "policy_loss: null pointer or ld=%lld < C=%d or no rows", (long long)ld, C);
+  LEC_CHECK_ARG(workspace && workspace_bytes >= kWorkBytes, "policy_loss: workspace needs %lld bytes", (long long)kWorkBytes);
+  LEC_CHECK_ARG(clip_low >= 0.0f && clip_high >= 0.0f, "policy_loss: clip bounds %g, %g are negative", (double)clip_low, (double)clip_high);
+  LEC_CHECK_ARG(kl_coef == 0.0f || ref_logp, "policy_loss: a KL coefficient needs the reference's log-probabilities");
+  hipStream_t st = (hipStream_t)stream;
+  unsigned int* counter = (unsigned int*)workspace;
+  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, counter, st);
+  if (rs != LEC_OK) return rs;
+  int LW = 1;
+  while (LW < L) LW <<= 1;
+  const int64_t n = R * G, per = 256 / LW, blocks = (n + per - 1) / per;
+  by_type(dtype, [&](auto* tag) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
+    hipLaunchKernelGGL((policy_kernel<T>), dim3((unsigned)(blocks > kMaxSumBlocks ? kMaxSumBlocks : blocks)), dim3(256), 0, st, (const T*)logits, ld, n, LW, t, paths, adv, old_logp,
+                       ref_logp, clip_low, clip_high, kl_coef, per_path, (const float2*)partials, coef, loss, stats, norm, (double*)((char*)workspace + 256), counter);
+  });
+  LEC_CHECK_LAUNCH("policy_kernel");
+  return LEC_OK;
+}

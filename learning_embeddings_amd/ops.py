@@ -320,6 +320,161 @@ class MultiLevelCEFn(torch.autograd.Function):
         return (ctx.g * gl).to(ctx.dt), None, None, None, None
 
 
+# ------------------------------------------------------------------------------------------------ feedback on label paths
+DTYPE_CODE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+MAX_PATH_LEVELS, MAX_PATHS_PER_ROW = 16, 64
+
+
+class PathLevels:
+    """The level sizes of a hierarchy in the form the C ABI takes them (host memory, read during the call)."""
+
+    def __init__(self, levels):
+        self.sizes = [int(v) for v in levels]
+        if not 1 <= len(self.sizes) <= MAX_PATH_LEVELS or min(self.sizes) < 1:
+            raise ValueError('levels must be 1 to %d sizes of at least one class, got %s' % (MAX_PATH_LEVELS, self.sizes))
+        self.L, self.C = len(self.sizes), sum(self.sizes)
+        self._arr = (C.c_int32 * self.L)(*self.sizes)
+        self.ptr = C.cast(self._arr, C.c_void_p)
+
+    @classmethod
+    def of(cls, levels):
+        """levels: a PathLevels, a labelmap (its `.levels`), or a sequence of sizes."""
+        return levels if isinstance(levels, cls) else cls(getattr(levels, 'levels', levels))
+
+
+def _path_logits(logits, levels):
+    """(kernel's view of the logits, dtype code, row stride): row-major with an element stride of one; rows may be strided (a slice of columns of a larger
+    matrix), a transposed or broadcast tensor is copied first."""
+    if not logits.is_cuda:
+        dptr(logits)                                                             # raises: there is no CPU fallback
+    if logits.dtype not in DTYPE_CODE:
+        raise TypeError('logits must be float32, bfloat16 or float16, got %s' % logits.dtype)
+    if logits.dim() != 2 or logits.shape[1] != levels.C:
+        raise ValueError('logits must be [rows, %d] (the sum of the levels), got %s' % (levels.C, tuple(logits.shape)))
+    z = logits
+    if z.stride(1) != 1 and z.shape[1] > 1 or z.stride(0) < z.shape[1] and z.shape[0] > 1:
+        z = z.contiguous()
+    return z, DTYPE_CODE[z.dtype], (z.stride(0) if z.shape[0] > 1 else z.shape[1])
+
+
+def _paths_arg(paths, shape, like):
+    if tuple(paths.shape) != tuple(shape):
+        raise ValueError('paths must be %s, got %s' % (tuple(shape), tuple(paths.shape)))
+    if paths.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8):
+        raise TypeError('paths must hold signed integers (the class within its level, negative = not known), got %s' % paths.dtype)
+    if paths.device != like.device:
+        raise ValueError('paths are on %s, the logits on %s' % (paths.device, like.device))
+    return paths.to(torch.int64).contiguous()
+
+
+def _entries_arg(t, name, shape, like):
+    """A constant of the loss, fp32 and contiguous (log-probabilities of another model, advantages); its gradient is not taken."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError('%s must be %s, got %s' % (name, tuple(shape), tuple(t.shape)))
+    if not t.is_floating_point():
+        raise TypeError('%s must be floating point, got %s' % (name, t.dtype))
+    if t.device != like.device:
+        raise ValueError('%s are on %s, the logits on %s' % (name, t.device, like.device))
+    return t.detach().to(torch.float32).contiguous()
+
+
+def _path_buffers(z, code, R, levels):
+    """One allocation a call: [workspace | partials].  Owned by the call (by its autograd node when a backward follows), so calls on other streams and captured
+    graphs share nothing."""
+    npart = lib.lec_path_partials_bytes(code, R, levels.C, levels.ptr, levels.L)
+    if npart < 0:
+        check(int(npart))
+    work = lib.lec_path_workspace_bytes()
+    buf = torch.empty(work + npart, dtype=torch.uint8, device=z.device)
+    return buf, C.c_void_p(buf.data_ptr()), work, C.c_void_p(buf.data_ptr() + work)
+
+
+def _path_backward(ctx, coef, up, norm_ptr):
+    z, paths, buf = ctx.saved_tensors[:3]
+    levels, code, ld, R, G, partials = ctx.meta
+    with torch.cuda.device(z.device):
+        dz = torch.empty(R, levels.C, dtype=z.dtype, device=z.device)
+        check(lib.lec_path_logp_bwd(dptr(z), code, ld, R, levels.C, levels.ptr, levels.L, dptr(paths), G, partials, dptr(coef), dptr(up), norm_ptr,
+                                    dptr(dz), levels.C, stream_ptr()))
+    return dz
+
+
+class PathLogProbFn(torch.autograd.Function):
+    """logp[r, g, l] of every entry of every path; gradient of the logits for any upstream gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, paths, levels):
+        z, code, ld = _path_logits(logits, levels)
+        R, G = paths.shape[:2]
+        with torch.cuda.device(z.device):
+            logp = torch.empty(R, G, levels.L, dtype=torch.float32, device=z.device)
+            if R == 0 or G == 0:
+                ctx.meta = None
+                ctx.empty = (tuple(logits.shape), logits.dtype, logits.device)
+                return logp
+            buf, _, work, partials = _path_buffers(z, code, R, levels)
+            check(lib.lec_path_logp_fwd(dptr(z), code, ld, R, levels.C, levels.ptr, levels.L, dptr(paths), G, dptr(logp), partials, stream_ptr()))
+        ctx.save_for_backward(z, paths, buf)
+        ctx.meta = (levels, code, ld, R, G, partials)
+        return logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        if ctx.meta is None:
+            shape, dtype, device = ctx.empty
+            return torch.zeros(shape, dtype=dtype, device=device), None, None
+        return _path_backward(ctx, g.to(torch.float32).contiguous(), None, None), None, None
+
+
+class PreferenceLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, paths, ref, levels, beta, smoothing, shared):
+        z, code, ld = _path_logits(logits, levels)
+        R = z.shape[0]
+        P, G = (R, 2) if shared else (R // 2, 1)
+        with torch.cuda.device(z.device):
+            loss = torch.empty((), dtype=torch.float32, device=z.device)
+            rewards = torch.empty(P, 2, dtype=torch.float32, device=z.device)
+            coef = torch.empty(R * G * levels.L, dtype=torch.float32, device=z.device)
+            buf, ws, work, partials = _path_buffers(z, code, R, levels)
+            check(lib.lec_preference_loss_fwd(dptr(z), code, ld, P, int(shared), levels.C, levels.ptr, levels.L, dptr(paths), dptr(ref), beta, smoothing,
+                                              dptr(loss), dptr(rewards), dptr(coef), partials, ws, work, stream_ptr()))
+        ctx.save_for_backward(z, paths, buf, coef)
+        ctx.meta = (levels, code, ld, R, G, partials)
+        ctx.mark_non_differentiable(rewards)
+        return loss, rewards
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gl, _gr):
+        return (_path_backward(ctx, ctx.saved_tensors[3], gl.to(torch.float32).contiguous(), None),) + (None,) * 6
+
+
+class PolicyLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, paths, adv, old, ref, levels, low, high, kl, per_path):
+        z, code, ld = _path_logits(logits, levels)
+        R, G = paths.shape[:2]
+        with torch.cuda.device(z.device):
+            loss = torch.empty((), dtype=torch.float32, device=z.device)
+            stats = torch.empty(2, dtype=torch.float32, device=z.device)
+            coef = torch.empty(4 + R * G * levels.L, dtype=torch.float32, device=z.device)              # norm, 3 unused | coefficients
+            buf, ws, work, partials = _path_buffers(z, code, R, levels)
+            check(lib.lec_policy_loss_fwd(dptr(z), code, ld, R, levels.C, levels.ptr, levels.L, dptr(paths), G, dptr(adv), dptr(old), dptr(ref), low, high, kl,
+                                          int(per_path), dptr(loss), dptr(stats), dptr(coef), C.c_void_p(coef.data_ptr() + 16), partials, ws, work, stream_ptr()))
+        ctx.save_for_backward(z, paths, buf, coef)
+        ctx.meta = (levels, code, ld, R, G, partials)
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gl, _gs):
+        coef = ctx.saved_tensors[3]
+        return (_path_backward(ctx, coef[4:], gl.to(torch.float32).contiguous(), dptr(coef)),) + (None,) * 9
+
+
 # ------------------------------------------------------------------------------------------------ per-model fusion records
 # The fused paths hand work from one autograd node to another: a convolution leaves the BatchNorm statistics of its output in the
 # BatchNorm workspace, a BatchNorm leaves pass 2 of its backward to the convolution behind it, ...  Each hand-off is a record keyed by

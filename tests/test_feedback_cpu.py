@@ -1,0 +1,150 @@
+"""Feedback operators without a GPU: the oracle against autograd and against differences, and every refusal of the host side."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import feedback_oracle as O
+
+
+def case(seed, R=5, G=3, levels=(2, 3, 7), known=0.7):
+    rs = np.random.RandomState(seed)
+    z = rs.randn(R, sum(levels)) * 2
+    paths = np.stack([rs.randint(0, n, size=(R, G)) for n in levels], 2)
+    paths[rs.rand(*paths.shape) > known] = -1
+    old, ref = O.path_log_probs(z, paths, levels) + 0.3 * rs.randn(*paths.shape), O.path_log_probs(z, paths, levels) + 0.3 * rs.randn(*paths.shape)
+    return z, paths, old, ref, rs.randn(R, G), list(levels)
+
+
+def torch_logp(z, paths, levels):
+    out = [torch.where(y >= 0, torch.log_softmax(zl, 1).gather(1, y.clamp(min=0)), torch.zeros((), dtype=z.dtype))
+           for zl, y in zip(z.split(levels, 1), torch.from_numpy(paths).unbind(2))]
+    return torch.stack(out, 2)
+
+
+def test_oracle_log_probs_and_gradient_against_autograd():
+    z, paths, _, _, _, lv = case(0)
+    coef = np.random.RandomState(1).randn(*paths.shape)
+    zt = torch.from_numpy(z).requires_grad_()
+    lp = torch_logp(zt, paths, lv)
+    (lp * torch.from_numpy(coef)).sum().backward()
+    assert np.abs(lp.detach().numpy() - O.path_log_probs(z, paths, lv)).max() < 1e-13
+    assert np.abs(zt.grad.numpy() - O.path_grad(z, paths, lv, coef)[0]).max() < 1e-13
+
+
+@pytest.mark.parametrize('shared', [True, False])
+def test_oracle_preference_gradient_against_differences(shared):
+    z, paths, _, ref, _, lv = case(2, R=6, G=2)
+    paths, ref = (paths, ref) if shared else (paths[:, 0], ref[:, 0])
+    f = lambda zz: O.preference_loss(zz, paths, ref, lv, 0.4, 0.1)[0]
+    coef = O.preference_loss(z, paths, ref, lv, 0.4, 0.1)[2]
+    g = O.path_grad(z, paths if shared else paths[:, None], lv, coef if shared else coef[:, None])[0]
+    v = np.random.RandomState(3).randn(*z.shape)
+    h = 1e-5                                                    # central differences: error h^2 f''' / 6 + 2^-52 / h, both below 1e-9
+    assert abs((f(z + h * v) - f(z - h * v)) / (2 * h) - (g * v).sum()) < 1e-9
+
+
+@pytest.mark.parametrize('reduction', ['level', 'path'])
+@pytest.mark.parametrize('with_old', [True, False])
+def test_oracle_policy_gradient_against_differences(reduction, with_old):
+    z, paths, old, ref, adv, lv = case(4)
+    old_c = old if with_old else None
+    coef = O.policy_loss(z, paths, adv, old_c, ref, lv, 0.2, 0.25, 0.1, reduction)[2]
+    g = O.path_grad(z, paths, lv, coef)[0]
+    base = O.path_log_probs(z, paths, lv)                       # on-policy: rho's gradient is taken at old = the present model, held fixed
+    f = lambda zz: O.policy_loss(zz, paths, adv, old if with_old else base, ref, lv, 0.2, 0.25, 0.1, reduction)[0]
+    v = np.random.RandomState(5).randn(*z.shape)
+    h = 1e-6
+    assert abs((f(z + h * v) - f(z - h * v)) / (2 * h) - (g * v).sum()) < 1e-8
+
+
+def test_oracle_policy_clips_both_ways_and_an_empty_batch_of_entries_is_zero():
+    z, paths, old, ref, adv, lv = case(6, known=1.0)
+    old = O.path_log_probs(z, paths, lv) - 1.0                  # rho = e: clipped where A > 0 only
+    _, stats, coef = O.policy_loss(z, paths, adv, old, ref, lv, 0.2, 0.2, 0.0, 'level')
+    assert abs(stats[1] - (adv > 0).mean()) < 1e-12 and (coef[adv > 0] == 0).all() and (coef[adv < 0] != 0).all()
+    loss, stats, coef = O.policy_loss(z, np.full_like(paths, -1), adv, old, ref, lv, 0.2, 0.2, 0.1, 'level')
+    assert loss == 0 and (stats == 0).all() and (coef == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def lm(levels=(2, 3)):
+    from learning_embeddings_amd.hierarchy import SyntheticLabelMap
+    return SyntheticLabelMap(list(levels))
+
+
+def test_levels_and_settings_are_checked():
+    from learning_embeddings_amd import loss, ops
+    for bad in ([], [3, 0], [1] * 17):
+        with pytest.raises(ValueError, match='levels'):
+            ops.PathLevels.of(bad)
+    with pytest.raises(ValueError, match='label_smoothing'):
+        loss.PreferenceLoss(lm(), label_smoothing=1.5)
+    with pytest.raises(ValueError, match='reduction'):
+        loss.ClippedPolicyLoss(lm(), reduction='sum')
+    with pytest.raises(ValueError, match='negative'):
+        loss.ClippedPolicyLoss(lm(), clip_low=-0.1)
+
+
+def test_shapes_types_and_devices_are_refused():
+    from learning_embeddings_amd import loss
+    z, lv = torch.zeros(4, 5), [2, 3]
+    y = torch.zeros(4, 2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        loss.path_log_probs(z, y, lv)
+    with pytest.raises(ValueError, match='paths must be'):
+        loss.path_log_probs(z, torch.zeros(4, 3, dtype=torch.int64), lv)
+    with pytest.raises(ValueError, match='outputs must be'):
+        loss.path_log_probs(z[0], y, lv)
+    with pytest.raises(TypeError, match='signed integers'):
+        loss.path_log_probs(z, y.float(), lv)
+    with pytest.raises(ValueError, match='at most 64 paths'):
+        loss.path_log_probs(z, torch.zeros(4, 65, 2, dtype=torch.int64), lv)
+    pref = loss.PreferenceLoss(lv)
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        pref(z, y, torch.zeros(4, 2))
+    with pytest.raises(ValueError, match='at least one pair'):
+        pref(z[:3], y[:3], torch.zeros(3, 2))
+    with pytest.raises(ValueError, match='at least one pair'):
+        pref(z[:0], y[:0], torch.zeros(0, 2))
+    with pytest.raises(ValueError, match='ref_log_probs must be'):
+        pref(z, y, torch.zeros(4))
+    with pytest.raises(TypeError, match='floating'):
+        pref(z, y, torch.zeros(4, 2, dtype=torch.int64))
+    pol = loss.ClippedPolicyLoss(lv, kl_coef=0.1)
+    with pytest.raises(ValueError, match='needs ref_log_probs'):
+        pol(z, y, torch.zeros(4))
+    pol = loss.ClippedPolicyLoss(lv)
+    with pytest.raises(ValueError, match='advantages must be'):
+        pol(z, y, torch.zeros(4, 2))
+    with pytest.raises(ValueError, match='at least one path'):
+        pol(z, torch.zeros(4, 0, 2, dtype=torch.int64), torch.zeros(4, 0))
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        pol(z, y, torch.zeros(4))
+
+
+def test_c_entries_report_bad_arguments():
+    import ctypes
+    from learning_embeddings_amd import _lib
+    lib = _lib.lib
+    def sizes(*v):
+        return ctypes.cast((ctypes.c_int32 * len(v))(*v), ctypes.c_void_p)
+    def err():
+        return lib.lec_last_error().decode()
+    assert lib.lec_path_partials_bytes(_lib.DTYPE_F32, 10, 5, sizes(2, 3), 2) == 10 * 2 * 8
+    assert lib.lec_path_partials_bytes(_lib.DTYPE_F32, 1, 2304, sizes(2304), 1) == 8             # one run of 64 lanes x 9 vectors x 4
+    assert lib.lec_path_partials_bytes(_lib.DTYPE_F32, 1, 2305, sizes(2305), 1) == 16
+    assert lib.lec_path_partials_bytes(_lib.DTYPE_BF16, 1, 2560, sizes(2560), 1) == 8
+    assert lib.lec_path_partials_bytes(_lib.DTYPE_F16, 1, 2561, sizes(2561), 1) == 16
+    for args, word in (((9, 1, 5, sizes(2, 3), 2), 'dtype'), ((0, 1, 5, sizes(2, 2), 2), 'sum to'), ((0, 1, 5, sizes(2, 4), 2), 'sum to'), ((0, 1, 5, sizes(5, 0), 2), 'empty level'),
+                       ((0, 1, 17, sizes(*[1] * 17), 17), 'levels'), ((0, -1, 5, sizes(2, 3), 2), 'rows')):
+        assert lib.lec_path_partials_bytes(*args) == _lib.E_ARG and word in err()
+    p = ctypes.c_void_p(256)                                    # never dereferenced: every call below is refused before its launch
+    assert lib.lec_path_logp_fwd(p, 0, 4, 1, 5, sizes(2, 3), 2, p, 1, p, p, None) == _lib.E_ARG and 'ld' in err()
+    assert lib.lec_path_logp_fwd(p, 0, 5, 1, 5, sizes(2, 3), 2, p, 65, p, p, None) == _lib.E_ARG and '1..64' in err()
+    assert lib.lec_path_logp_fwd(None, 0, 5, 1, 5, sizes(2, 3), 2, p, 1, p, p, None) == _lib.E_ARG
+    assert lib.lec_path_logp_bwd(p, 0, 5, 1, 5, sizes(2, 3), 2, p, 1, p, p, None, None, p, 4, None) == _lib.E_ARG
+    w = lib.lec_path_workspace_bytes()
+    assert lib.lec_preference_loss_fwd(p, 0, 5, 1, 1, 5, sizes(2, 3), 2, p, p, 0.1, 0.0, p, p, p, p, p, w - 1, None) == _lib.E_ARG and 'workspace' in err()
+    assert lib.lec_preference_loss_fwd(p, 0, 5, 1, 1, 5, sizes(2, 3), 2, p, p, 0.1, 1.5, p, p, p, p, p, w, None) == _lib.E_ARG and 'label_smoothing' in err()
+    assert lib.lec_policy_loss_fwd(p, 0, 5, 1, 5, sizes(2, 3), 2, p, 1, p, None, None, 0.2, 0.2, 0.1, 0, p, p, p, p, p, p, w, None) == _lib.E_ARG and 'KL' in err()
+    assert lib.lec_policy_loss_fwd(p, 0, 5, 1, 5, sizes(2, 3), 2, p, 1, p, None, None, -0.2, 0.2, 0.0, 0, p, p, p, p, p, p, w, None) == _lib.E_ARG and 'negative' in err()

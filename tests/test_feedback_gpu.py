@@ -1,0 +1,350 @@
+"""Feedback operators on the MI355X against the 64-bit oracle: values, gradients, masks, strides, streams, graphs.
+
+Tolerances, from the arithmetic (u = 2^-24, one rounding to 32 bits):
+  * a softmax term exp(z - m): the difference, its product with log2 e and the constant round by u each, relative error 3 |z - m| u, plus 2 u of the exponential;
+    the mean of |z - m| under the softmax is at most log n, the sum's chain is at most 40 + 6 + 24 additions: relative error of the sum below (3 log n + 80) u;
+  * logp in 64 bits from that sum, rounded once: LT(n) = (3 log n + 90) u, plus u |logp|;
+  * a probability: (3 |z - m| + 3 log n + 90) u relative;
+  * a coefficient follows from logp in 64 bits: its error is the formula's derivative times LT, plus u of itself;
+  * the gradient's elements round once to the logits' type: half a step, eps / 2 relative (fp16 also 2^-25 absolute below its normal range)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import feedback_oracle as O
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DT = {'fp32': torch.float32, 'bf16': torch.bfloat16, 'fp16': torch.float16}
+ETHEC = [6, 21, 135, 561]
+S5 = [2, 8, 32, 128, 512, 2048, 8192, 39078]
+LEVELS = {'one': [1], 'two': [2], 'ones': [1, 1, 1], 'odd': [3, 5], 'ethec': ETHEC, 'sixteen': list(range(1, 17)), 'run32': [2303, 2304, 2305], 'run16': [2559, 2560, 2561],
+          'wide': [4608, 5121, 7], 's5': S5}
+
+
+def LT(levels):
+    return np.array([(3 * np.log(n) + 90) * U for n in levels])
+
+
+def make(levels, R, G, dtype, seed=0, known=0.8):
+    """z in the type under test (as float64 too), paths, old, ref, adv: an entry's ratio stays off both clip bounds by 1e-3."""
+    rs = np.random.RandomState(seed)
+    z = torch.from_numpy((rs.randn(R, sum(levels)) * 2.5).astype(np.float32)).to(DT[dtype])
+    zd = z.double().numpy()
+    paths = np.stack([rs.randint(0, n, size=(R, G)) for n in levels], 2)
+    paths[rs.rand(*paths.shape) > known] = -1
+    if R > 2:
+        paths[1] = -1                                           # a row with nothing known
+        paths[2] = paths[2, :1]                                 # a row whose paths are all the same
+    lp = O.path_log_probs(zd, paths, levels)
+    d = 0.25 * rs.randn(*lp.shape)
+    for b in (0.8, 1.2):
+        d[np.abs(np.exp(d) - b) < 1e-3] += 0.004
+    old, ref = (lp - d), lp + 0.3 * rs.randn(*lp.shape)
+    old, ref = old.astype(np.float32), ref.astype(np.float32)
+    return z, zd, paths, old, ref, rs.randn(R, G).astype(np.float32)
+
+
+def dev(a):
+    return (torch.from_numpy(a) if isinstance(a, np.ndarray) else a).cuda()
+
+
+def check_grad(got, z, zd, paths, levels, coef, coef_err, dtype):
+    want, size = O.path_grad(zd, paths, levels, coef)
+    _, err = O.path_grad(zd, paths, levels, coef_err)
+    tol = np.zeros_like(want)
+    for l, (a, b) in enumerate(O.level_slices(levels)):
+        span = zd[:, a:b].max(1, keepdims=True) - zd[:, a:b]
+        tol[:, a:b] = (3 * span + 3 * np.log(b - a) + 100) * U * size[:, a:b] + err[:, a:b]
+    tol += torch.finfo(DT[dtype]).eps / 2 * (np.abs(want) + tol) + (2.0 ** -25 if dtype == 'fp16' else 1e-37)
+    g = got.double().cpu().numpy()
+    assert g.shape == want.shape and got.dtype == DT[dtype]
+    bad = ~(np.abs(g - want) <= tol)
+    assert not bad.any(), 'max error / tolerance %.3g at %s' % ((np.abs(g - want) / tol).max(), np.argwhere(bad)[0])
+    return g
+
+
+SHAPES = [('one', 1, 1), ('two', 3, 1), ('ones', 4, 2), ('odd', 5, 3), ('ethec', 1, 1), ('ethec', 37, 8), ('sixteen', 9, 5), ('run32', 3, 2), ('run16', 3, 2), ('wide', 4, 3),
+          ('ethec', 3, 64), ('s5', 3, 2)]
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('name,R,G', SHAPES)
+def test_path_log_probs(name, R, G, dtype):
+    from learning_embeddings_amd import loss
+    lv = LEVELS[name]
+    z, zd, paths, _, _, _ = make(lv, R, G, dtype)
+    zt = dev(z).requires_grad_()
+    lp = loss.path_log_probs(zt, dev(paths), lv)
+    want = O.path_log_probs(zd, paths, lv)
+    assert lp.dtype == torch.float32 and lp.shape == paths.shape
+    assert (np.abs(lp.detach().cpu().numpy() - want) <= LT(lv) + U * np.abs(want)).all()
+    assert (lp.detach().cpu().numpy()[paths < 0] == 0).all()
+    up = np.random.RandomState(9).randn(*paths.shape).astype(np.float32)
+    lp.backward(dev(up))
+    check_grad(zt.grad, z, zd, paths, lv, up.astype(np.float64), 2 * U * G * np.abs(up), dtype)
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('shared', [True, False])
+@pytest.mark.parametrize('name,P', [('one', 1), ('odd', 5), ('ethec', 1), ('ethec', 33), ('sixteen', 9), ('wide', 4), ('s5', 2)])
+@pytest.mark.parametrize('smooth', [0.0, 0.1])
+def test_preference_loss(name, P, shared, dtype, smooth):
+    from learning_embeddings_amd import loss
+    lv = LEVELS[name]
+    R, G = (P, 2) if shared else (2 * P, 1)
+    z, zd, paths, _, ref, _ = make(lv, R, G, dtype, seed=3)
+    p, rf = (paths, ref) if shared else (paths[:, 0], ref[:, 0])
+    beta = 0.5
+    zt = dev(z).requires_grad_()
+    l, rewards = loss.PreferenceLoss(lv, beta=beta, label_smoothing=smooth)(zt, dev(p), dev(rf))
+    assert not rewards.requires_grad
+    want, r, coef = O.preference_loss(zd, p, rf.astype(np.float64), lv, beta, smooth)
+    ed = beta * 2 * LT(lv).sum()
+    assert abs(float(l) - want) <= ed + 2 * U * abs(want)
+    assert (np.abs(rewards.cpu().numpy() - r) <= ed + U * np.abs(r)).all()
+    l.backward()
+    cerr = (beta / P * (ed / 4 + 2 * U) + 4 * U * np.abs(coef)) * (p >= 0)
+    full = (lambda a: a) if shared else (lambda a: a[:, None])
+    check_grad(zt.grad, z, zd, paths, lv, full(coef), full(cerr), dtype)
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('name,R,G', SHAPES)
+@pytest.mark.parametrize('reduction,kl,with_old', [('level', 0.1, True), ('path', 0.0, True), ('path', 0.1, False)])
+def test_policy_loss(name, R, G, dtype, reduction, kl, with_old):
+    from learning_embeddings_amd import loss
+    lv = LEVELS[name]
+    z, zd, paths, old, ref, adv = make(lv, R, G, dtype, seed=5)
+    zt = dev(z).requires_grad_()
+    crit = loss.ClippedPolicyLoss(lv, clip_low=0.2, clip_high=0.2, kl_coef=kl, reduction=reduction)
+    l, stats = crit(zt, dev(paths), dev(adv), dev(old) if with_old else None, dev(ref) if kl else None)
+    o64, r64 = (old.astype(np.float64) if with_old else None), (ref.astype(np.float64) if kl else None)
+    want, st, coef = O.policy_loss(zd, paths, adv, o64, r64, lv, 0.2, 0.2, kl, reduction)
+    on = paths >= 0
+    w = on / max(on.sum(), 1) if reduction == 'level' else on / np.maximum(on.sum(2, keepdims=True), 1) / (R * G)
+    lp = O.path_log_probs(zd, paths, lv)
+    rho = np.exp(np.where(on, lp - old, 0)) if with_old else np.ones(lp.shape)
+    q = np.where(on, ref - lp, 0) if kl else np.zeros(lp.shape)
+    A = np.abs(adv.astype(np.float64))[:, :, None]
+    e_t = w * LT(lv) * (rho * A + kl * (np.exp(q) + 1))
+    mag = (w * (rho * A + kl * np.abs(np.expm1(q) - q))).sum()
+    assert abs(float(l) - want) <= e_t.sum() + 4 * U * mag
+    assert abs(float(stats[0]) - st[0]) <= (w * LT(lv) * (np.exp(q) + 1)).sum() + 4 * U * st[0]
+    assert abs(float(stats[1]) - st[1]) <= 4 * U
+    l.backward()
+    cerr = w * LT(lv) * (rho * A + kl * np.exp(q)) + 8 * U * G * np.abs(coef)
+    check_grad(zt.grad, z, zd, paths, lv, coef, cerr, dtype)
+
+
+def test_gradient_against_differences_of_the_kernels_own_loss():
+    """Directional derivative, h = 2^-6: truncation h^2 / 6 times the third derivative along v (|v| <= 1 element-wise, 4 levels, beta 0.5: below 4, so 2e-4), and the two
+    losses' errors (LT of four levels, beta 0.5: 4e-5) over 2 h: 3e-3.  The derivative itself is of order 0.1."""
+    from learning_embeddings_amd import loss
+    z, zd, paths, _, ref, _ = make(ETHEC, 6, 2, 'fp32', seed=11, known=1.0)
+    crit = loss.PreferenceLoss(ETHEC, beta=0.5)
+    v = torch.from_numpy(np.random.RandomState(12).uniform(-1, 1, size=z.shape).astype(np.float32)).cuda()
+    zt = dev(z).requires_grad_()
+    crit(zt, dev(paths), dev(ref))[0].backward()
+    h = 2.0 ** -6
+    with torch.no_grad():
+        d = (float(crit(zt + h * v, dev(paths), dev(ref))[0]) - float(crit(zt - h * v, dev(paths), dev(ref))[0])) / (2 * h)
+    assert abs(d - float((zt.grad * v).sum())) < 4e-3
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+def test_levels_nobody_counts_may_hold_anything(dtype):
+    from learning_embeddings_amd import loss
+    z, zd, paths, old, ref, adv = make(ETHEC, 7, 3, dtype, seed=7, known=1.0)
+    paths[:, :, 2] = -1; paths[3] = -1
+    clean = dev(z).requires_grad_()
+    dirty_z = z.clone()
+    dirty_z[:, 27:162] = float('nan'); dirty_z[3] = float('inf')
+    dirty = dev(dirty_z).requires_grad_()
+    old2, ref2 = old.copy(), ref.copy()
+    old2[paths < 0] = np.nan; ref2[paths < 0] = np.inf
+    crit = loss.ClippedPolicyLoss(ETHEC, kl_coef=0.1)
+    a, sa = crit(clean, dev(paths), dev(adv), dev(old), dev(ref)); a.backward()
+    b, sb = crit(dirty, dev(paths), dev(adv), dev(old2), dev(ref2)); b.backward()
+    assert torch.isfinite(a) and torch.equal(a, b) and torch.equal(sa, sb)
+    assert torch.equal(clean.grad, dirty.grad)
+    assert (dirty.grad[:, 27:162] == 0).all() and (dirty.grad[3] == 0).all()
+
+
+def test_nothing_counted_at_all():
+    from learning_embeddings_amd import loss
+    z = torch.full((4, sum(ETHEC)), float('nan'), device='cuda', requires_grad=True)
+    none = torch.full((4, 2, 4), -1, device='cuda')
+    e = torch.full((4, 2, 4), float('nan'), device='cuda')
+    for red in ('level', 'path'):
+        z.grad = None
+        l, st = loss.ClippedPolicyLoss(ETHEC, kl_coef=0.1, reduction=red)(z, none, torch.ones(4, 2, device='cuda'), e, e)
+        l.backward()
+        assert float(l) == 0 and (st == 0).all() and (z.grad == 0).all()
+    z.grad = None
+    l, r = loss.PreferenceLoss(ETHEC)(z, none, e)
+    l.backward()
+    assert abs(float(l) - np.log(2)) <= 2 * U and (r == 0).all() and (z.grad == 0).all()
+
+
+def test_excluded_classes_and_special_values():
+    """-inf (or the type's lowest value) takes a class out of its softmax; a counted class that is out has logp -inf; a level with nothing in, a NaN or a +inf gives NaN;
+    a class that the level does not have gives NaN and reads nothing; other rows are as without."""
+    from learning_embeddings_amd import loss
+    lv = [4, 700]
+    z, zd, _, _, _, _ = make(lv, 8, 1, 'fp32', seed=1)
+    z[0, 1:4] = -float('inf'); z[1, 4:704] = -float('inf'); z[2, 5] = float('nan'); z[3, 6] = float('inf'); z[4, 1:3] = torch.finfo(torch.float32).min
+    zd = z.double().numpy()
+    paths = np.zeros((8, 1, 2), dtype=np.int64)
+    paths[5, 0, 1] = 700; paths[6, 0, 0] = 2 ** 40; paths[7, 0, 1] = -2 ** 40
+    zt = dev(z).requires_grad_()
+    lp = loss.path_log_probs(zt, dev(paths), lv)
+    lp.backward(torch.ones_like(lp))
+    got, g = lp.detach().cpu().numpy()[:, 0], zt.grad.cpu().numpy()
+    want = O.path_log_probs(zd, paths, lv)[:, 0]
+    nan = np.zeros((8, 2), dtype=bool); nan[[1, 2, 3, 5], 1] = True; nan[6, 0] = True
+    assert (np.isnan(got) == nan).all() and (np.abs(got - want)[~nan] <= (LT(lv) + U * np.abs(want))[~nan]).all()
+    assert got[7, 1] == 0 and got[0, 0] == 0
+    for r in range(8):
+        for l, (a, b) in enumerate(O.level_slices(lv)):
+            assert np.isfinite(g[r, a:b]).all() == (not nan[r, l]), (r, l)
+    assert (g[0, 1:4] == 0).all() and (g[4, 1:3] == 0).all() and (g[7, 4:] == 0).all()
+    out = torch.zeros(1, 704, device='cuda'); out[0, 0] = -float('inf')
+    assert float(loss.path_log_probs(out, torch.zeros(1, 2, dtype=torch.int64, device='cuda'), lv)[0, 0]) == -float('inf')
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+def test_strided_transposed_and_broadcast_logits(dtype):
+    from learning_embeddings_amd import loss
+    lv = [3, 5, 600]
+    z, zd, paths, _, _, _ = make(lv, 6, 2, dtype, seed=2)
+    y = dev(paths)
+    base = dev(z)
+    plain = base.clone().requires_grad_()
+    ref = loss.path_log_probs(plain, y, lv); ref.sum().backward()
+    for off in (0, 1, 3):                                       # a slice of columns: odd offset, odd row stride
+        big = torch.full((6, 613 + off), float('nan'), dtype=z.dtype, device='cuda')
+        big[:, off:off + 608] = base
+        big.requires_grad_()
+        lp = loss.path_log_probs(big[:, off:off + 608], y, lv); lp.sum().backward()
+        assert torch.equal(lp, ref) and torch.equal(big.grad[:, off:off + 608], plain.grad) and (big.grad[:, :off] == 0).all() and (big.grad[:, off + 608:] == 0).all()
+    tr = base.t().contiguous().requires_grad_()
+    lp = loss.path_log_probs(tr.t(), y, lv); lp.sum().backward()
+    assert torch.equal(lp, ref) and torch.equal(tr.grad, plain.grad.t())
+    every = base.flip(0)[::2].contiguous()                      # strided rows and strided paths
+    big = base.flip(0)
+    lp = loss.path_log_probs(big[::2], y[::2], lv)
+    assert torch.equal(lp, loss.path_log_probs(every, y[::2].contiguous(), lv))
+    row = base[:1].clone().requires_grad_()                     # one row for all paths: its gradient is the sum over the rows
+    lp = loss.path_log_probs(row.expand(6, -1), y, lv); lp.sum().backward()
+    want, size = O.path_grad(np.repeat(zd[:1], 6, 0), paths, lv, np.ones(paths.shape))
+    half = torch.finfo(z.dtype).eps / 2
+    assert (np.abs(row.grad.double().cpu().numpy()[0] - want.sum(0)) <= (200 * U + 7 * half) * size.sum(0) + 2.0 ** -22).all()
+
+
+def test_scaled_and_summed_upstream_and_two_uses_of_one_tensor():
+    from learning_embeddings_amd import loss
+    z, zd, paths, old, ref, adv = make(ETHEC, 9, 2, 'fp32', seed=8)
+    crit = loss.PreferenceLoss(ETHEC); pol = loss.ClippedPolicyLoss(ETHEC, kl_coef=0.05)
+    a = dev(z).requires_grad_(); crit(a, dev(paths), dev(ref))[0].backward()
+    b = dev(z).requires_grad_(); pol(b, dev(paths), dev(adv), dev(old), dev(ref))[0].backward()
+    c = dev(z).requires_grad_()
+    l = 0.5 * crit(c, dev(paths), dev(ref))[0] + 2.0 * pol(c, dev(paths), dev(adv), dev(old), dev(ref))[0]
+    l.backward(retain_graph=True)
+    want = 0.5 * a.grad + 2.0 * b.grad
+    tol = 8 * U * (0.5 * a.grad.abs() + 2.0 * b.grad.abs())
+    assert ((c.grad - want).abs() <= tol + 1e-30).all()
+    first = c.grad.clone(); c.grad = None
+    l.backward()                                                # a second backward of the same graph
+    assert torch.equal(first, c.grad)
+    l, _ = crit(c, dev(paths), dev(ref))
+    l += 1.0                                                    # the value may be changed in place, the inputs of the backward may not
+    l.backward()
+    l, _ = crit(c * 1.0, dev(paths), dev(ref))
+    y = c * 1.0
+    l, _ = crit(y, dev(paths), dev(ref))
+    y.mul_(2.0)
+    with pytest.raises(RuntimeError, match='inplace'):
+        l.backward()
+
+
+def test_empty_batches_and_int32_paths():
+    from learning_embeddings_amd import loss
+    z = torch.zeros(0, sum(ETHEC), device='cuda', requires_grad=True)
+    lp = loss.path_log_probs(z, torch.zeros(0, 4, dtype=torch.int64, device='cuda'), ETHEC)
+    assert lp.shape == (0, 4)
+    lp.sum().backward()
+    assert z.grad.shape == z.shape
+    z = torch.randn(3, sum(ETHEC), device='cuda', requires_grad=True)
+    lp = loss.path_log_probs(z, torch.zeros(3, 0, 4, dtype=torch.int64, device='cuda'), ETHEC)
+    assert lp.shape == (3, 0, 4)
+    lp.sum().backward()
+    assert (z.grad == 0).all()
+    y = torch.tensor([[0, 1, 2, 3]] * 3, device='cuda')
+    assert torch.equal(loss.path_log_probs(z, y, ETHEC), loss.path_log_probs(z, y.int(), ETHEC))
+    with pytest.raises(ValueError, match='logits on'):
+        loss.path_log_probs(z, y.cpu(), ETHEC)
+    with pytest.raises(TypeError, match='float32, bfloat16 or float16'):
+        loss.path_log_probs(z.double(), y, ETHEC)
+
+
+def test_many_rows_give_the_same_bits_every_time_and_on_another_stream():
+    from learning_embeddings_amd import loss
+    g = torch.Generator(device='cuda').manual_seed(0)
+    z = torch.randn(3001, sum(ETHEC), generator=g, device='cuda').requires_grad_()
+    y = torch.stack([torch.randint(-1, n, (3001, 5), generator=g, device='cuda') for n in ETHEC], 2)
+    e = torch.randn(3001, 5, 4, generator=g, device='cuda') - 5
+    adv = torch.randn(3001, 5, generator=g, device='cuda')
+    crit = loss.ClippedPolicyLoss(ETHEC, kl_coef=0.01)
+    def once():
+        z.grad = None
+        l, st = crit(z, y, adv, e, e); l.backward()
+        return l.detach().clone(), st.clone(), z.grad.clone()
+    a, b = once(), once()
+    s = torch.cuda.Stream(); s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        c = once()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for other in (b, c):
+        assert all(torch.equal(u, v) for u, v in zip(a, other))
+
+
+@pytest.mark.parametrize('which', ['pref', 'policy', 'logp'])
+def test_captured_and_replayed(which):
+    """Two graphs captured on one stream share no buffer: replayed in turn and out of order, between eager work, each equals the eager result."""
+    from learning_embeddings_amd import loss
+    z, zd, paths, old, ref, adv = make(ETHEC, 40, 2, 'fp32', seed=13)
+    y, o, r, a = dev(paths), dev(old), dev(ref), dev(adv)
+    pref, pol = loss.PreferenceLoss(ETHEC), loss.ClippedPolicyLoss(ETHEC, kl_coef=0.1)
+    def step(zz):
+        zz = zz.detach().requires_grad_()
+        if which == 'pref':
+            v = pref(zz, y, r)[0]
+        elif which == 'policy':
+            v = pol(zz, y, a, o, r)[0]
+        else:
+            v = (loss.path_log_probs(zz, y, ETHEC) * o).sum(2).amax()
+        g, = torch.autograd.grad(v, zz)
+        return v.detach(), g
+    inputs = [dev(z).clone(), dev(z).clone()]
+    s = torch.cuda.Stream(); s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(inputs[0])
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [], []
+    for x in inputs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            outs.append(step(x))
+        graphs.append(gr)
+    gen = torch.Generator(device='cuda').manual_seed(5)
+    for k in range(4):
+        for x in inputs:
+            x.normal_(generator=gen)
+        want = [step(x) for x in inputs]
+        for i in ((0, 1), (1, 0), (1, 1), (0, 0))[k]:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in set(((0, 1), (1, 0), (1, 1), (0, 0))[k]):
+            assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
