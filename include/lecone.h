@@ -283,6 +283,25 @@ int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t R, in
                         float* norm, float* coef, void* partials, void* workspace, int64_t workspace_bytes, lec_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * (6c) Microscaled 4-bit floating point (MXFP4): quantisation, its inverse, the product of a frozen classifier head.  No counterpart in the reference.
+ *      Blocks of 32 elements along a row share X = 2^clamp(floor(log2 max|v|) - 2, -127, 127), kept as the byte log2 X + 127; an element is v / X rounded to
+ *      nearest (ties to even) into {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign, saturating.  A block with a NaN or an infinity: byte 255, stands for NaN.
+ *      codes:  [ceil(rows / 16)][ceil(k / 128)][64 lanes][16 bytes]: lane l holds row l % 16, elements 32 (l / 16) .. + 32 of the tile, low nibble first
+ *      scales: [ceil(rows / 16)][ceil(k / 512)][64 lanes][4 bytes]:  lane l's scale bytes of four consecutive 128-element tiles
+ *      Padding is zero.  Both 16-byte aligned, lec_mxfp4_{codes,scales}_bytes() long (negative: bad sizes; rows <= 2^31 - 16, k <= 2^24).
+ *      x: [rows, k] of `dtype`, row stride ld >= k, element-aligned.  dequantize writes fp32 or bf16 (both exact).
+ *      linear: y[M, N] (ydtype, ldy) = x_4 w_4^T + bias; x is quantised by the call into `workspace` (lec_mxfp4_linear_workspace_bytes, one call in flight per
+ *      workspace), products are exact, sums 32-bit in a fixed order, bias (fp32 [N] or NULL) is added in 32 bits, one rounding to ydtype.
+ * ------------------------------------------------------------------------------------------------------------- */
+int64_t lec_mxfp4_codes_bytes(int64_t rows, int64_t k);
+int64_t lec_mxfp4_scales_bytes(int64_t rows, int64_t k);
+int lec_mxfp4_quantize(const void* x, int dtype, int64_t ld, int64_t rows, int64_t k, void* codes, void* scales, lec_stream_t stream);
+int lec_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t k, void* out, int dtype, int64_t ld, lec_stream_t stream);
+int64_t lec_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t k);
+int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t M, const void* wcodes, const void* wscales, int64_t N, int64_t k, const float* bias,
+                     void* y, int ydtype, int64_t ldy, void* workspace, int64_t workspace_bytes, lec_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * (7) Fused BatchNorm (+ residual add) (+ ReLU) on NHWC bf16 activations -- the HBM-bound half of the ResNet backbone
  *     behind FeatCNN18 / FeatCNN (oe_h.py:311,317 -> torchvision BasicBlock/Bottleneck: `relu(bn(conv(x)))`,
  *     `relu(bn(conv(x)) + identity)`, downsample `bn(conv(x))`) and their autograd.

@@ -5,7 +5,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('LEC_LIB_PATH') or os.path.join(_HERE, 'liblecone.so')     # LEC_LIB_PATH: A/B builds of the same ABI
-ABI_VERSION = 34
+ABI_VERSION = 35
 
 OK, E_ARG, E_HIP, E_EMPTY, E_STATE = 0, -1, -2, -3, -4
 ENERGY_HYP_CONE, ENERGY_ORDER, ENERGY_EUC_CONE = 0, 1, 2
@@ -81,6 +81,12 @@ def _load():
         'lec_path_logp_bwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p, p, p, i64, p]),
         'lec_preference_loss_fwd': (i32, [p, i32, i64, i64, i32, i32, p, i32, p, p, f32, f32, p, p, p, p, p, i64, p]),
         'lec_policy_loss_fwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p, f32, f32, f32, i32, p, p, p, p, p, p, i64, p]),
+        'lec_mxfp4_codes_bytes': (i64, [i64, i64]),
+        'lec_mxfp4_scales_bytes': (i64, [i64, i64]),
+        'lec_mxfp4_quantize': (i32, [p, i32, i64, i64, i64, p, p, p]),
+        'lec_mxfp4_dequantize': (i32, [p, p, i64, i64, p, i32, i64, p]),
+        'lec_mxfp4_linear_workspace_bytes': (i64, [i64, i64, i64]),
+        'lec_mxfp4_linear': (i32, [p, i32, i64, i64, p, p, i64, i64, p, p, i32, i64, p, i64, p]),
         'lec_bn_workspace_bytes': (i64, [i32]),
         'lec_bn_fwd': (i32, [p, p, i64, i32, p, p, f32, f32, p, p, i32, p, p, p, i32, p, p, i64, p]),
         'lec_bn_bwd': (i32, [p, p, p, p, p, i64, i32, p, p, p, p, p, p, p, i32, p, i64, i32, p]),

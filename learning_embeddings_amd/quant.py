@@ -1,0 +1,127 @@
+"""Microscaled 4-bit floating point (MXFP4) and a classifier head held in it.  No counterpart in the reference.
+
+Blocks of 32 elements along a row share a power of two, 2^(floor(log2 max|v|) - 2) within [2^-127, 2^127]; an element is one of
+{0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign times it, rounded to nearest with ties to even, saturating.  A block that holds a NaN or an
+infinity stands for NaN.  17/32 bytes an element (rows padded to 16, elements to 128, scale words to 512).
+
+    head = MXFP4Linear.from_linear(model.fc)          # quantises the weights once
+    logits = head(features)                           # quantises the features row by row, multiplies on the 4-bit matrix cores, sums in 32 bits
+
+The head is frozen -- a reference model's, or one that serves: its weights take no gradient and it passes none to its input."""
+import ctypes as C
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from ._lib import lib, check, dptr, stream_ptr
+from .ops import DTYPE_CODE
+
+
+def _matrix(x, name):
+    """(row-major 2-D view, dtype code, row stride)"""
+    if x.dtype not in DTYPE_CODE:
+        raise TypeError('%s must be float32, bfloat16 or float16, got %s' % (name, x.dtype))
+    if not x.is_cuda:
+        dptr(x)                                                                  # raises: there is no CPU fallback
+    if x.stride(1) != 1 and x.shape[1] > 1 or x.stride(0) < x.shape[1] and x.shape[0] > 1:
+        x = x.contiguous()
+    return x, DTYPE_CODE[x.dtype], (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+
+
+class MXFP4Tensor:
+    """A matrix [rows, k] in 4 bits: `codes` and `scales` (uint8, in the matrix instruction's tile order -- see include/lecone.h) on one device."""
+
+    def __init__(self, codes, scales, shape):
+        self.codes, self.scales, self.shape = codes, scales, tuple(int(v) for v in shape)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def dequantize(self, dtype=torch.float32):
+        """The values it stands for, [rows, k]; float32 and bfloat16 hold every one of them exactly."""
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError('the values are exact in float32 and bfloat16 only, got %s' % dtype)
+        rows, k = self.shape
+        out = torch.empty(rows, k, dtype=dtype, device=self.device)
+        if rows and k:
+            with torch.cuda.device(self.device):
+                check(lib.lec_mxfp4_dequantize(dptr(self.codes), dptr(self.scales), rows, k, dptr(out), DTYPE_CODE[dtype], k, stream_ptr()))
+        return out
+
+
+def mxfp4_quantize(x):
+    """x [rows, k] (float32 / bfloat16 / float16) -> MXFP4Tensor.  Carries no gradient."""
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError('x must be [rows, k] with k > 0, got %s' % (tuple(x.shape),))
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError('mxfp4_quantize passes no gradient to its input: detach it, or call it under torch.no_grad()')
+    z, code, ld = _matrix(x, 'x')
+    rows, k = z.shape
+    if rows == 0:
+        e = torch.empty(0, dtype=torch.uint8, device=z.device)
+        return MXFP4Tensor(e, e, (0, k))
+    with torch.cuda.device(z.device):
+        codes = torch.empty(_size(lib.lec_mxfp4_codes_bytes(rows, k)), dtype=torch.uint8, device=z.device)
+        scales = torch.empty(_size(lib.lec_mxfp4_scales_bytes(rows, k)), dtype=torch.uint8, device=z.device)
+        check(lib.lec_mxfp4_quantize(dptr(z), code, ld, rows, k, dptr(codes), dptr(scales), stream_ptr()))
+    return MXFP4Tensor(codes, scales, (rows, k))
+
+
+def _size(n):
+    if n < 0:
+        raise ValueError('matrix too large for the 4-bit form (at most 2^31 - 16 rows of 2^24 elements)')
+    return int(n)
+
+
+class MXFP4Linear(nn.Module):
+    """y = x_4 W_4^T + b with the weights held, and x quantised on the way in, in 4 bits; sums in 32 bits, one rounding to the output's type.
+    weight [out_features, in_features], bias [out_features] or None; out_dtype None: the input's.  Frozen: see above."""
+
+    def __init__(self, weight, bias=None, out_dtype=None):
+        super().__init__()
+        if out_dtype is not None and out_dtype not in DTYPE_CODE:
+            raise TypeError('out_dtype must be float32, bfloat16 or float16, got %s' % out_dtype)
+        q = mxfp4_quantize(weight.detach())
+        if q.shape[0] == 0:
+            raise ValueError('weight must have at least one row')
+        self.out_features, self.in_features = q.shape
+        self.out_dtype = out_dtype
+        if bias is not None and tuple(bias.shape) != (self.out_features,):
+            raise ValueError('bias must be [%d], got %s' % (self.out_features, tuple(bias.shape)))
+        self.register_buffer('codes', q.codes)
+        self.register_buffer('scales', q.scales)
+        self.register_buffer('bias', None if bias is None else bias.detach().to(device=q.device, dtype=torch.float32).contiguous().clone())
+
+    @classmethod
+    def from_linear(cls, linear, out_dtype=None):
+        return cls(linear.weight, linear.bias, out_dtype)
+
+    def extra_repr(self):
+        return 'in_features=%d, out_features=%d, bias=%s, out_dtype=%s' % (self.in_features, self.out_features, self.bias is not None, self.out_dtype)
+
+    def dequantize(self, dtype=torch.float32):
+        return MXFP4Tensor(self.codes, self.scales, (self.out_features, self.in_features)).dequantize(dtype)
+
+    def forward(self, x):
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError('MXFP4Linear is a frozen head and passes no gradient to its input: call it under torch.no_grad(), or on a detached input')
+        if x.dim() == 0 or x.shape[-1] != self.in_features:
+            raise ValueError('x must be [..., %d], got %s' % (self.in_features, tuple(x.shape)))
+        if x.device != self.codes.device:
+            raise ValueError('x is on %s, the head on %s' % (x.device, self.codes.device))
+        z, code, ld = _matrix(x.reshape(-1, self.in_features), 'x')
+        M, N, k = z.shape[0], self.out_features, self.in_features
+        dtype = self.out_dtype or x.dtype
+        with torch.cuda.device(z.device):
+            y = torch.empty(M, N, dtype=dtype, device=z.device)
+            if M:
+                ws = torch.empty(_size(lib.lec_mxfp4_linear_workspace_bytes(M, N, k)), dtype=torch.uint8, device=z.device)      # this call's own
+                b = self.bias if self.bias is None or self.bias.dtype == torch.float32 else self.bias.float()     # (.half() on a model converts its buffers)
+                check(lib.lec_mxfp4_linear(dptr(z), code, ld, M, dptr(self.codes), dptr(self.scales), N, k, dptr(b), dptr(y), DTYPE_CODE[dtype], N, dptr(ws), ws.numel(),
+                                           stream_ptr()))
+        return y.view(*x.shape[:-1], N)

@@ -98,3 +98,29 @@ def policy_loss(z, paths, adv, old, ref, levels, low, high, kl, reduction):
     loss = (w * (kl * k3 - gain)).sum()
     coef = w * (np.where(clipped, 0.0, -rho * A) - kl * np.expm1(q))
     return loss, np.array([(w * k3).sum(), (w * clipped).sum()]), coef
+
+
+# ------------------------------------------------------------------------------------------------ 4-bit microscaled form
+E2M1 = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def mxfp4_values(x):
+    """The values the 4-bit form of x [rows, k] stands for: per block of 32 the power of two, then the nearest of the eight magnitudes (the one
+    with the even code on a tie), 6 beyond the last."""
+    x = np.asarray(x, dtype=np.float64)
+    rows, k = x.shape
+    out = np.empty((rows, k))
+    for a in range(0, k, 32):
+        v = x[:, a:a + 32]
+        top = np.abs(v).max(1)
+        bad = ~np.isfinite(top)
+        _, e = np.frexp(np.where(bad | (top == 0), 1.0, top))
+        X = np.where(top == 0, -127, np.clip(e - 3, -127, 127))
+        s = np.ldexp(1.0, X)[:, None]
+        q = np.abs(np.where(bad[:, None], 0.0, v)) / s
+        d = np.abs(q[:, :, None] - E2M1)
+        best = d.min(2, keepdims=True)
+        near = d == best                                        # one code, or two neighbours of which one is even
+        code = np.where(near.sum(2) > 1, (near * (np.arange(8) % 2 == 0)).argmax(2), near.argmax(2))
+        out[:, a:a + 32] = np.where(bad[:, None], np.nan, np.copysign(E2M1[code] * s, v))
+    return out

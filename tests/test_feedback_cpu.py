@@ -148,3 +148,47 @@ def test_c_entries_report_bad_arguments():
     assert lib.lec_preference_loss_fwd(p, 0, 5, 1, 1, 5, sizes(2, 3), 2, p, p, 0.1, 1.5, p, p, p, p, p, w, None) == _lib.E_ARG and 'label_smoothing' in err()
     assert lib.lec_policy_loss_fwd(p, 0, 5, 1, 5, sizes(2, 3), 2, p, 1, p, None, None, 0.2, 0.2, 0.1, 0, p, p, p, p, p, p, w, None) == _lib.E_ARG and 'KL' in err()
     assert lib.lec_policy_loss_fwd(p, 0, 5, 1, 5, sizes(2, 3), 2, p, 1, p, None, None, -0.2, 0.2, 0.0, 0, p, p, p, p, p, p, w, None) == _lib.E_ARG and 'negative' in err()
+
+
+# ------------------------------------------------------------------------------------------------ 4-bit form
+def test_oracle_mxfp4_rounding_by_hand():
+    v = np.array([[0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9, 0.2501, -0.7499, -5.0001, 6.0, 4.0] + [0.0] * 19])
+    want = [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0, 0.5, -0.5, -6.0, 6.0, 4.0] + [0.0] * 19
+    assert O.mxfp4_values(v)[0].tolist() == want
+    assert (O.mxfp4_values(v * 2.0 ** 40)[0] == np.array(want) * 2.0 ** 40).all()
+    assert (O.mxfp4_values(np.full((1, 33), 3.99)) == 3.0).all()         # 3.99 / 2^-1 = 7.98 saturates: 6 x 2^-1, in the full block and in the short one
+    assert np.isnan(O.mxfp4_values(np.array([[1.0] * 31 + [np.inf] + [1.0]]))).tolist() == [[True] * 32 + [False]]
+    assert (O.mxfp4_values(np.full((1, 32), 2.0 ** -149)) == 0).all() and (O.mxfp4_values(np.full((1, 32), 2.0 ** -128)) == 2.0 ** -128).all()
+
+def test_mxfp4_refusals():
+    import torch.nn as nn
+    from learning_embeddings_amd import _lib, quant
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        quant.mxfp4_quantize(torch.zeros(4, 32))
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        quant.MXFP4Linear.from_linear(nn.Linear(32, 4))
+    with pytest.raises(ValueError, match=r'\[rows, k\]'):
+        quant.mxfp4_quantize(torch.zeros(4))
+    with pytest.raises(ValueError, match=r'\[rows, k\]'):
+        quant.mxfp4_quantize(torch.zeros(4, 0))
+    with pytest.raises(TypeError, match='float32, bfloat16 or float16'):
+        quant.mxfp4_quantize(torch.zeros(4, 32, dtype=torch.float64))
+    with pytest.raises(RuntimeError, match='no gradient'):
+        quant.mxfp4_quantize(torch.zeros(4, 32, requires_grad=True))
+    with pytest.raises(TypeError, match='out_dtype'):
+        quant.MXFP4Linear(torch.zeros(4, 32), out_dtype=torch.float64)
+    e = torch.zeros(0, dtype=torch.uint8)
+    with pytest.raises(TypeError, match='exact'):
+        quant.MXFP4Tensor(e, e, (0, 32)).dequantize(torch.float16)
+    lib = _lib.lib
+    assert lib.lec_mxfp4_codes_bytes(1, 1) == 1024 and lib.lec_mxfp4_codes_bytes(17, 129) == 4096 and lib.lec_mxfp4_scales_bytes(17, 513) == 1024
+    assert lib.lec_mxfp4_codes_bytes(2 ** 31 - 16, 128) == 2 ** 27 * 1024 - 1024 and lib.lec_mxfp4_codes_bytes(0, 1) < 0 and lib.lec_mxfp4_codes_bytes(2 ** 31, 1) < 0
+    assert lib.lec_mxfp4_codes_bytes(1, 2 ** 24 + 1) < 0 and lib.lec_mxfp4_linear_workspace_bytes(1, 0, 32) < 0
+    import ctypes
+    p = ctypes.c_void_p(256)
+    assert lib.lec_mxfp4_quantize(p, 0, 31, 1, 32, p, p, None) == _lib.E_ARG and b'ld' in lib.lec_last_error()
+    assert lib.lec_mxfp4_quantize(p, 7, 32, 1, 32, p, p, None) == _lib.E_ARG and b'dtype' in lib.lec_last_error()
+    assert lib.lec_mxfp4_dequantize(p, p, 1, 32, p, _lib.DTYPE_F16, 32, None) == _lib.E_ARG
+    assert lib.lec_mxfp4_linear(p, 0, 32, 1, p, p, 4, 32, None, p, 0, 3, p, 1 << 20, None) == _lib.E_ARG and b'ldy' in lib.lec_last_error()
+    assert lib.lec_mxfp4_linear(p, 0, 32, 1, p, p, 4, 32, None, p, 0, 4, p, 1024, None) == _lib.E_ARG and b'workspace' in lib.lec_last_error()
+    assert lib.lec_mxfp4_linear(p, 0, 32, 1, p, p, 4, 32, None, p, 5, 4, p, 1 << 20, None) == _lib.E_ARG and b'dtype' in lib.lec_last_error()
