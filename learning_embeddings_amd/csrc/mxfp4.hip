@@ -29,97 +29,106 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
 template <> __device__ __forceinline__ _Float16 from_f32<_Float16>(float v) { return (_Float16)v; }
 
-// 32 elements at x (n of them exist) -> 32 codes and the scale byte
+// 8 elements at x (n of them exist), one load of 16 or 32 bytes at element alignment
 template <typename T>
-__device__ __forceinline__ uint4 quantize_block(const T* __restrict__ x, int n, unsigned int& scale) {
-  float v[32];
-  if (n >= 32) {
-    T raw[32];
-    __builtin_memcpy(raw, (const void*)x, sizeof(raw));          // 16-byte loads at element alignment
+__device__ __forceinline__ void load8(const T* __restrict__ x, int n, float (&v)[8]) {
+  if (n >= 8) {
+    T raw[8];
+    __builtin_memcpy(raw, (const void*)x, sizeof(raw));
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = to_f32(raw[i]);
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = i < n ? to_f32(x[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(x[i]) : 0.0f;
   }
-  unsigned int top = 0;                                          // as integers: a NaN is above infinity, infinity above every number
-#pragma unroll
-  for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  const int e = (int)(top >> 23);                                // floor(log2 max) = e - 127 (0 for subnormals, whose byte is clamped to 0 anyway)
-  if (e == 255) { scale = 255u; return make_uint4(0u, 0u, 0u, 0u); }
-  scale = (unsigned int)max(e - 2, 0);
-  const float inv = __uint_as_float((254u - scale) << 23);       // 1 / X, exact
-  unsigned int w[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    w[q] = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float f = v[q * 8 + j];
-      const float a = fabsf(f) * inv;                            // exact (or far below the first threshold), < 8
-      const float magic = a < 2.0f ? 6291456.0f : (a < 4.0f ? 12582912.0f : 25165824.0f);      // 1.5 * 2^23 * the spacing: the sum rounds to a multiple of it, ties to even
-      const float r = (a + magic) - magic;
-      const int code = min(r < 2.0f ? (int)(2.0f * r) : (r < 4.0f ? (int)r + 2 : (int)(0.5f * r) + 4), 7);
-      w[q] |= (unsigned int)(code | ((__float_as_uint(f) >> 28) & 8u)) << (4 * j);
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One wave a row tile and a group of four k tiles (a scale word).
+// Four neighbouring lanes hold a block, 8 elements each -> the lane's 8 codes and the block's scale byte.  The conversion instruction rounds to nearest even and
+// saturates; it is given v / X (a product with a power of two, exact or far below the first threshold) and the scale 1, so that X = 2^-127 needs no special case.
+__device__ __forceinline__ unsigned int quantize8(const float (&v)[8], unsigned int& scale) {
+  int top = 0;                                                   // as integers: a NaN is above infinity, infinity above every number
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, (int)(__float_as_uint(v[i]) & 0x7fffffffu));
+  top = max(top, __builtin_amdgcn_update_dpp(0, top, 0xB1, 0xf, 0xf, false));       // quad_perm: lane xor 1
+  top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x4E, 0xf, 0xf, false));       // lane xor 2
+  const int e = top >> 23;                                       // floor(log2 max) = e - 127 (0 for subnormals, whose byte is clamped to 0 anyway)
+  scale = e == 255 ? 255u : (unsigned int)max(e - 2, 0);
+  const float inv = __uint_as_float(e == 255 ? 0u : (254u - scale) << 23);          // 1 / X
+  unsigned int w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0] * inv, v[1] * inv, 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2] * inv, v[3] * inv, 1.0f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4] * inv, v[5] * inv, 1.0f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6] * inv, v[7] * inv, 1.0f, 3);
+  return e == 255 ? 0u : w;
+}
+
+// A block takes a row tile and a group of four k tiles (16 rows x 512 elements, one scale word a lane of the layout); a wave reads 512 consecutive elements of a row at
+// a time, 16 bytes a lane, so memory sees contiguous kilobytes; the codes of 16 rows meet in the L2.
 template <typename T>
-__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int K, int KT, int KG, int64_t ntask, uint4* __restrict__ codes,
+__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int K, int KT, int KG, int64_t ntask, unsigned int* __restrict__ codes,
                                                              unsigned int* __restrict__ scales) {
-  const int lane = threadIdx.x & 63, r = lane & 15, kb = lane >> 4;
-  const int64_t nwave = (int64_t)gridDim.x * 4;
-  for (int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); task < ntask; task += nwave) {
+  __shared__ unsigned char s_scale[256];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int ktl = lane >> 4, kb = (lane >> 2) & 3, sub = lane & 3;
+  for (int64_t task = blockIdx.x; task < ntask; task += gridDim.x) {
     const int64_t rt = task / KG;
-    const int kg = (int)(task - rt * KG);
-    const int64_t row = rt * 16 + r;
-    unsigned int word = 0;
+    const int kg = (int)(task - rt * KG), k = kg * 512 + lane * 8, kt = kg * 4 + ktl;
+    float v[4][8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int kt = kg * 4 + i;
-      if (kt >= KT) break;
-      const int k = kt * 128 + kb * 32;
-      unsigned int s = 0;
-      uint4 c = make_uint4(0u, 0u, 0u, 0u);
-      if (row < rows && k < K) c = quantize_block(x + row * ld + k, K - k, s);
-      codes[(rt * KT + kt) * 64 + lane] = c;
-      word |= s << (8 * i);
+      const int64_t row = rt * 16 + wave * 4 + i;
+      load8(x + row * ld + k, row < rows ? K - k : 0, v[i]);
     }
-    scales[(rt * KG + kg) * 64 + lane] = word;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = wave * 4 + i;
+      unsigned int sc;
+      const unsigned int w = quantize8(v[i], sc);
+      if (kt < KT) codes[((rt * KT + kt) * 64 + kb * 16 + r) * 4 + sub] = w;
+      if (sub == 0) s_scale[(kb * 16 + r) * 4 + ktl] = (unsigned char)sc;
+    }
+    __syncthreads();
+    if (t < 64) scales[(rt * KG + kg) * 64 + t] = ((const unsigned int*)s_scale)[t];
+    __syncthreads();                                             // (the next task writes s_scale)
   }
 }
 
-__device__ __forceinline__ float decode(unsigned int code, int scale) {
-  const float mag[8] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f};
-  const float v = ldexpf(mag[code & 7u], scale - 127);
-  return scale == 255 ? __builtin_nanf("") : ((code & 8u) ? -v : v);
-}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <typename T>
-__global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const uint4* __restrict__ codes, const unsigned char* __restrict__ scales, int64_t rows, int K, int KT, int KG,
+__global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const unsigned int* __restrict__ codes, const unsigned char* __restrict__ scales, int64_t rows, int K, int KT, int KG,
                                                                int64_t ntask, T* __restrict__ out, int64_t ld) {
-  const int lane = threadIdx.x & 63, r = lane & 15, kb = lane >> 4;
-  const int64_t nwave = (int64_t)gridDim.x * 4;
-  for (int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); task < ntask; task += nwave) {
-    const int64_t rt = task / KT;
-    const int kt = (int)(task - rt * KT);
-    const int64_t row = rt * 16 + r;
-    const int k = kt * 128 + kb * 32;
-    if (row >= rows || k >= K) continue;
-    const uint4 c = codes[(rt * KT + kt) * 64 + lane];
-    const int s = scales[((rt * KG + (kt >> 2)) * 64 + lane) * 4 + (kt & 3)];
-    const unsigned int w[4] = {c.x, c.y, c.z, c.w};
-    T v[32];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int ktl = lane >> 4, kb = (lane >> 2) & 3, sub = lane & 3;
+  for (int64_t task = blockIdx.x; task < ntask; task += gridDim.x) {
+    const int64_t rt = task / KG;
+    const int kg = (int)(task - rt * KG), k = kg * 512 + lane * 8, kt = kg * 4 + ktl;
+    if (k >= K) continue;
+    unsigned int w[4], sc[4];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = from_f32<T>(decode(w[i >> 3] >> (4 * (i & 7)), s));
-    T* o = out + row * ld + k;
-    if (k + 32 <= K) __builtin_memcpy((void*)o, v, sizeof(v));
-    else {
+    for (int i = 0; i < 4; ++i) {
+      const int r = wave * 4 + i;                                // (rows past the end are padding of the same tile)
+      w[i] = codes[((rt * KT + kt) * 64 + kb * 16 + r) * 4 + sub];
+      sc[i] = scales[((rt * KG + kg) * 64 + kb * 16 + r) * 4 + ktl];
+    }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) if (k + i < K) o[i] = v[i];
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = rt * 16 + wave * 4 + i;
+      if (row >= rows) continue;
+      const float X = sc[i] == 255u ? __builtin_nanf("") : (sc[i] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(sc[i] << 23));      // 2^(byte - 127); byte 0: subnormal
+      T v[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x2 f = j == 0 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 0) : j == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 1)
+                      : j == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 2) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 3);
+        v[2 * j] = from_f32<T>(f.x * X); v[2 * j + 1] = from_f32<T>(f.y * X);
+      }
+      T* o = out + row * ld + k;
+      if (k + 8 <= K) __builtin_memcpy((void*)o, v, sizeof(v));
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (k + j < K) o[j] = v[j];
+      }
     }
   }
 }
@@ -135,13 +144,87 @@ __device__ __forceinline__ f32x4 mfma4(const uint4& a, const uint4& b, f32x4 c, 
 }
 
 // y[m, n] = sum_k x[m, k] w[n, k] + bias[n].  The weights are the A operand: a lane's four accumulators are four consecutive classes n of one row m.
-// A wave owns NT x MT tiles, a block 2 x 2 waves; operands straight from memory (every load is a contiguous kilobyte).
-template <typename T, int NT, int MT>
-__global__ __launch_bounds__(256) void mxfp4_linear_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
-                                                           const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nt0 = ((int)blockIdx.x * 2 + (wave & 1)) * NT, ntn = (N + 15) >> 4;
-  const int64_t mt0 = ((int64_t)blockIdx.y * 2 + (wave >> 1)) * MT, mtn = (M + 15) >> 4;
+template <typename T>
+__device__ __forceinline__ void store4(T* __restrict__ y, int64_t ldy, int64_t M, int N, int64_t m, int n, const f32x4& acc, const float (&bv)[4]) {
+  if (m >= M || n >= N) return;
+  T o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(acc[e] + bv[e]);
+  T* p = y + m * ldy + n;
+  if (n + 4 <= N) __builtin_memcpy((void*)p, o, sizeof(o));
+  else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (n + e < N) p[e] = o[e];
+  }
+}
+__device__ __forceinline__ void load_bias(const float* __restrict__ bias, int N, int n, float (&bv)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bv[e] = bias && n + e < N ? bias[n + e] : 0.0f;
+}
+
+// At most 16 rows (one tile of x): the time is the weights' way from memory.  A wave owns one tile of 16 classes and asks for 16 k tiles of its weights at once; while
+// they are under way the block quantises x into LDS (each block again: x is small and comes from the L2, a launch of its own would cost more).  x has to fit 64 KB of LDS: K <= 7680.
+template <typename TX, typename T>
+__global__ __launch_bounds__(256) void mxfp4_linear_rows_kernel(const TX* __restrict__ x, int64_t ldx, int M, const uint4* __restrict__ wc, const unsigned int* __restrict__ wsc, int N, int K,
+                                                                int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned int* xcodes = (unsigned int*)smem;                    // [KT][64][4] words
+  unsigned char* xscale = smem + (size_t)KT * 1024;              // [KG][64][4] bytes
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int nt = min((int)blockIdx.x * 4 + wave, ((N + 15) >> 4) - 1);
+  const bool mine = (int)blockIdx.x * 4 + wave == nt;            // (a wave past the last tile repeats it and stores nothing)
+  constexpr int CH = 16;
+  uint4 w[CH];
+  unsigned int sw[CH / 4];
+  auto fetch = [&](int kt0) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) if (kt0 + i < KT) w[i] = wc[((int64_t)nt * KT + kt0 + i) * 64 + lane];
+#pragma unroll
+    for (int i = 0; i < CH / 4; ++i) if (kt0 / 4 + i < KG) sw[i] = wsc[((int64_t)nt * KG + kt0 / 4 + i) * 64 + lane];
+  };
+  fetch(0);
+  for (int i = t; i < KT * 64; i += 256) ((uint4*)xcodes)[i] = make_uint4(0u, 0u, 0u, 0u);       // rows that do not exist
+  for (int i = t; i < KG * 64; i += 256) ((unsigned int*)xscale)[i] = 0u;
+  __syncthreads();
+  const int per_row = KG * 64;                                   // 8-element pieces of a row, padded to whole groups of 512
+  for (int i = t; i < M * per_row; i += 256) {
+    const int r = i / per_row, q = i - r * per_row, k = q * 8, kt = k >> 7, kb = (k >> 5) & 3, sub = (k >> 3) & 3;
+    float v[8];
+    load8(x + (int64_t)r * ldx + k, K - k, v);
+    unsigned int sc;
+    const unsigned int c = quantize8(v, sc);
+    if (kt < KT) xcodes[(kt * 64 + kb * 16 + r) * 4 + sub] = c;
+    if (sub == 0) xscale[((kt >> 2) * 64 + kb * 16 + r) * 4 + (kt & 3)] = (unsigned char)sc;
+  }
+  __syncthreads();
+  f32x4 acc[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};                // two chains: an MFMA need not wait for the one before
+  for (int kt0 = 0; kt0 < KT; kt0 += CH) {
+    if (kt0) fetch(kt0);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      if (kt0 + i < KT) {
+        const uint4 b = ((const uint4*)xcodes)[(kt0 + i) * 64 + lane];
+        const unsigned int sb = ((const unsigned int*)xscale)[((kt0 + i) >> 2) * 64 + lane];
+        acc[i & 1] = mfma4(w[i], b, acc[i & 1], i & 3, sw[i >> 2], sb);
+      }
+    }
+  }
+  if (!mine) return;
+  const int n = nt * 16 + 4 * (lane >> 4);
+  float bv[4];
+  load_bias(bias, N, n, bv);
+  store4(y, ldy, M, N, lane & 15, n, acc[0] + acc[1], bv);
+}
+
+// A block of WN x WM waves, a wave NT x MT tiles, operands straight from memory (every load is a contiguous kilobyte): few tiles, or shapes too small for the ring below.
+template <typename T, int WN, int WM, int NT, int MT>
+__global__ __launch_bounds__(64 * WN * WM) void mxfp4_linear_small_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
+                                                                          const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y,
+                                                                          int64_t ldy) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nt0 = ((int)blockIdx.x * WN + wave % WN) * NT, ntn = (N + 15) >> 4;
+  const int64_t mt0 = ((int64_t)blockIdx.y * WM + wave / WN) * MT, mtn = (M + 15) >> 4;
+  if (nt0 >= ntn || mt0 >= mtn) return;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -172,23 +255,153 @@ __global__ __launch_bounds__(256) void mxfp4_linear_kernel(const uint4* __restri
   for (int i = 0; i < NT; ++i) {
     const int n = (nt0 + i) * 16 + 4 * (lane >> 4);
     float bv[4];
+    load_bias(bias, N, n, bv);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bv[e] = bias && n + e < N ? bias[n + e] : 0.0f;
+    for (int j = 0; j < MT; ++j) store4(y, ldy, M, N, (mt0 + j) * 16 + (lane & 15), n, acc[i][j], bv);
+  }
+}
+
+// Large products.  A block of 2 x 2 waves owns 256 x 256 of y, a wave 128 x 128 (8 x 8 tiles, 256 accumulators: one wave a SIMD, one block a CU).  A k tile of both operands is
+// 32 KB; a ring of four stages in LDS is filled by LDS-DMA (a wave's request is one contiguous kilobyte = one operand tile in lane order, so there is nothing to swizzle), three stages
+// ahead.  Per k tile a wave issues 64 MFMAs of 16 cycles and reads 16 KB of LDS: 96 KB of LDS traffic per 1024 cycles a CU, under its 128 B / clk.
+typedef __attribute__((address_space(3))) void lds_ptr;
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t make_rsrc(const void* p, unsigned bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00020000); }
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); __builtin_amdgcn_s_barrier(); asm volatile("" ::: "memory"); }
+
+// (A body with restrict parameters, inlined into the kernel: its memory accesses then carry alias scopes, without which the compiler waits for every outstanding
+// LDS-DMA before any read of LDS -- the ring would be one stage deep.)
+template <typename T>
+__device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
+                                                                  const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy,
+                                                                  int nbn, int nbm, int per_xcd) {
+  constexpr int STAGE = 32 * 1024, IPW = 8;                      // bytes of a stage; LDS-DMA instructions a wave issues for one
+  constexpr int PIN = (int)0x80000000;                           // a volatile load: it stays where it is written, ahead of the requests behind it
+  constexpr int OOB = 0x40000000;                                // past any operand buffer (KT <= 32 768: at most 2^29 bytes)
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave & 1, wm = wave >> 1;
+  // consecutive blocks land on the eight XCDs in turn: give each XCD a contiguous run of tiles, four tiles of rows by all tiles of classes at a time, so that a run's
+  // operands stay in its L2
+  const int64_t g = (int64_t)((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
+  if (g >= (int64_t)nbn * nbm) return;
+  const int band = (int)(g / (4 * (int64_t)nbn)), inb = (int)(g - (int64_t)band * 4 * nbn), bw = min(4, nbm - band * 4);
+  const int bn = __builtin_amdgcn_readfirstlane(inb / bw), bm = __builtin_amdgcn_readfirstlane(band * 4 + inb % bw);      // (the division leaves them in vector registers)
+  const int ntn = (N + 15) >> 4, mtn = (int)((M + 15) >> 4);
+  // The block's operand tiles of each side and their scales as buffers that end with the last of them; a tile past the matrix repeats the last one (and is not stored).
+  const int na_ = min(16, ntn - bn * 16), nb_ = min(16, mtn - bm * 16);
+  const rsrc_t ra = make_rsrc(wc + (int64_t)bn * 16 * KT * 64, (unsigned)na_ * KT * 1024), rb = make_rsrc(xc + (int64_t)bm * 16 * KT * 64, (unsigned)nb_ * KT * 1024);
+  const rsrc_t rsa = make_rsrc(wsc + (int64_t)bn * 16 * KG * 64, (unsigned)na_ * KG * 256), rsb = make_rsrc(xs + (int64_t)bm * 16 * KG * 64, (unsigned)nb_ * KG * 256);
+  auto issue = [&](int kt) {                                     // this wave's tiles of stage kt: 4 of the weights, 4 of x.  Past the last stage: no traffic, zeros in LDS
+    unsigned char* base = smem + (kt & 3) * STAGE + wave * 1024;
+    const int voff = lane * 16 + (kt < KT ? 0 : OOB), kc = min(kt, KT - 1);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const int64_t m = (mt0 + j) * 16 + (lane & 15);
-      if (m >= M || n >= N) continue;
-      T o[4];
+    for (int u = 0; u < 4; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr*)(base + u * 4096), 16, voff, (min(wave + 4 * u, na_ - 1) * KT + kc) * 1024, 0, 0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(acc[i][j][e] + bv[e]);
-      T* p = y + m * ldy + n;
-      if (n + 4 <= N) __builtin_memcpy((void*)p, o, sizeof(o));
-      else {
+    for (int u = 0; u < 4; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr*)(base + 16384 + u * 4096), 16, voff, (min(wave + 4 * u, nb_ - 1) * KT + kc) * 1024, 0, 0);
+  };
+  f32x4 acc[8][8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (n + e < N) p[e] = o[e];
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  int sa[8], sb[8], na[8], nb[8];                                // scale words: of this group of four k tiles, of the next one
+  auto fetch_scales = [&](int kg) {                              // (a group past the end: the last one again)
+    const int kc = min(kg, KG - 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      na[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, lane * 4, (min(wn * 8 + i, na_ - 1) * KG + kc) * 256, PIN);
+      nb[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, lane * 4, (min(wm * 8 + i, nb_ - 1) * KG + kc) * 256, PIN);
+    }
+  };
+  const uint4* A = (const uint4*)smem + wn * 512 + lane;         // this wave's operand tiles of slot 0
+  const uint4* B = (const uint4*)(smem + 16384) + wm * 512 + lane;
+  fetch_scales(0);
+  issue(0); issue(1); issue(2); issue(3);
+  wait_vm<3 * IPW>();                                            // stage 0 has landed for this wave ...
+  meet();                                                        // ... and for every wave
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    sa[i] = na[i]; sb[i] = nb[i];
+    asm volatile("" : "+v"(sa[i]), "+v"(sb[i]));                  // in registers before the loop: its own waits then count the loop's requests only
+  }
+  uint4 a = A[0], b[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b[j] = B[j * 64];
+  // One k tile: rows 0 .. 3 of the products run while the wave reads its other weights of the stage; then everybody is done reading stage kt, whose slot takes stage kt + 4, and
+  // stage kt + 1 has landed once at most the two younger stages' requests are outstanding (scale loads in between only make the wait stricter); rows 4 .. 7 run while
+  // stage kt + 1's first operands are read.  The order is pinned: left alone the scheduler puts every read before the first product.  Groups of four k tiles, the last one
+  // filled up with stages of zeros, so that the body has no branch.
+  auto tile = [&](int kt, auto qc) {
+    constexpr int q = decltype(qc)::value;
+    const uint4* Ao = A + q * (STAGE / 16);
+    const uint4* An = A + ((q + 1) & 3) * (STAGE / 16);
+    const uint4* Bn = B + ((q + 1) & 3) * (STAGE / 16);
+    uint4 ar[8], bx[8];
+    ar[0] = a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ar[i + 1] = Ao[(i + 1) * 64];
+      if (i > 0) ar[i + 4] = Ao[(i + 4) * 64];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][j] = mfma4(ar[i], b[j], acc[i][j], q, sa[i], sb[j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_vm<2 * IPW>();
+    meet();
+    if (q == 0) fetch_scales((kt >> 2) + 1);
+    issue(kt + 4);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 4; i < 8; ++i) {
+      if (i == 4) a = An[0];
+      bx[2 * (i - 4)] = Bn[2 * (i - 4) * 64];
+      bx[2 * (i - 4) + 1] = Bn[(2 * (i - 4) + 1) * 64];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][j] = mfma4(ar[i], b[j], acc[i][j], q, sa[i], sb[j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = bx[j];
+  };
+  for (int kt = 0; kt < KT; kt += 4) {
+    tile(kt, std::integral_constant<int, 0>{});
+    tile(kt + 1, std::integral_constant<int, 1>{});
+    tile(kt + 2, std::integral_constant<int, 2>{});
+    tile(kt + 3, std::integral_constant<int, 3>{});
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { sa[i] = na[i]; sb[i] = nb[i]; }
+  }
+  wait_vm<0>();                                                  // (the stages of zeros past the end still write LDS)
+  const rsrc_t rbias = make_rsrc(bias, bias ? (unsigned)N * 4u : 0u);
+  const bool inside = (bn + 1) * 256 <= N && (int64_t)(bm + 1) * 256 <= M;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = (bn * 16 + wn * 8 + i) * 16 + 4 * (lane >> 4);
+    float bv[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bv[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rbias, (n + e) * 4, 0, 0));       // (past the end: 0)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t m = (int64_t)(bm * 16 + wm * 8 + j) * 16 + (lane & 15);
+      if (inside) {
+        T o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(acc[i][j][e] + bv[e]);
+        __builtin_memcpy((void*)(y + m * ldy + n), o, sizeof(o));
+      } else {
+        store4(y, ldy, M, N, m, n, acc[i][j], bv);
       }
     }
   }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 1) void mxfp4_linear_big_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
+                                                                  const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy,
+                                                                  int nbn, int nbm, int per_xcd) {
+  mxfp4_linear_big_body<T>(xc, xs, M, wc, wsc, N, KT, KG, bias, y, ldy, nbn, nbm, per_xcd);
 }
 
 template <typename F> static int by_dtype(int dtype, const char* what, F&& f) {
@@ -200,14 +413,14 @@ template <typename F> static int by_dtype(int dtype, const char* what, F&& f) {
   set_error("%s: unknown dtype %d", what, dtype);
   return LEC_E_ARG;
 }
-static unsigned grid_of(int64_t waves) { const int64_t b = ceil_div(waves, 4); return (unsigned)(b > (1 << 22) ? (1 << 22) : b); }
+static unsigned grid_of(int64_t blocks) { return (unsigned)(blocks > (1 << 22) ? (1 << 22) : blocks); }
 
 static int quantize(const void* x, int dtype, int64_t ld, int64_t rows, int K, void* codes, void* scales, hipStream_t st) {
   const int KT = (int)ceil_div(K, 128), KG = (int)ceil_div(K, 512);
   const int64_t ntask = ceil_div(rows, 16) * KG;
   const int rc = by_dtype(dtype, "mxfp4_quantize", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    hipLaunchKernelGGL((mxfp4_quantize_kernel<T>), dim3(grid_of(ntask)), dim3(256), 0, st, (const T*)x, ld, rows, K, KT, KG, ntask, (uint4*)codes, (unsigned int*)scales);
+    hipLaunchKernelGGL((mxfp4_quantize_kernel<T>), dim3(grid_of(ntask)), dim3(256), 0, st, (const T*)x, ld, rows, K, KT, KG, ntask, (unsigned int*)codes, (unsigned int*)scales);
   });
   if (rc != LEC_OK) return rc;
   LEC_CHECK_LAUNCH("mxfp4_quantize_kernel");
@@ -234,12 +447,12 @@ extern "C" int lec_mxfp4_dequantize(const void* codes, const void* scales, int64
   LEC_CHECK_ARG(out && codes && scales && ld >= k, "mxfp4_dequantize: null pointer or ld=%lld < k=%lld", (long long)ld, (long long)k);
   LEC_CHECK_ARG(dtype == LEC_DTYPE_F32 || dtype == LEC_DTYPE_BF16, "mxfp4_dequantize: dtype %d does not hold every value (fp32 or bf16)", dtype);
   const int KT = (int)ceil_div(k, 128), KG = (int)ceil_div(k, 512);
-  const int64_t ntask = ceil_div(rows, 16) * KT;
+  const int64_t ntask = ceil_div(rows, 16) * KG;
   if (dtype == LEC_DTYPE_F32)
-    hipLaunchKernelGGL((mxfp4_dequantize_kernel<float>), dim3(grid_of(ntask)), dim3(256), 0, (hipStream_t)stream, (const uint4*)codes, (const unsigned char*)scales, rows, (int)k, KT, KG,
+    hipLaunchKernelGGL((mxfp4_dequantize_kernel<float>), dim3(grid_of(ntask)), dim3(256), 0, (hipStream_t)stream, (const unsigned int*)codes, (const unsigned char*)scales, rows, (int)k, KT, KG,
                        ntask, (float*)out, ld);
   else
-    hipLaunchKernelGGL((mxfp4_dequantize_kernel<__hip_bfloat16>), dim3(grid_of(ntask)), dim3(256), 0, (hipStream_t)stream, (const uint4*)codes, (const unsigned char*)scales, rows, (int)k,
+    hipLaunchKernelGGL((mxfp4_dequantize_kernel<__hip_bfloat16>), dim3(grid_of(ntask)), dim3(256), 0, (hipStream_t)stream, (const unsigned int*)codes, (const unsigned char*)scales, rows, (int)k,
                        KT, KG, ntask, (__hip_bfloat16*)out, ld);
   LEC_CHECK_LAUNCH("mxfp4_dequantize_kernel");
   return LEC_OK;
@@ -257,18 +470,56 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
   const int64_t need = codes_bytes(M, k) + scales_bytes(M, k);
   LEC_CHECK_ARG(workspace && workspace_bytes >= need, "mxfp4_linear: workspace needs %lld bytes", (long long)need);
   LEC_CHECK_ARG(ydtype == LEC_DTYPE_F32 || ydtype == LEC_DTYPE_BF16 || ydtype == LEC_DTYPE_F16, "mxfp4_linear: unknown dtype %d", ydtype);
+  LEC_CHECK_ARG(xdtype == LEC_DTYPE_F32 || xdtype == LEC_DTYPE_BF16 || xdtype == LEC_DTYPE_F16, "mxfp4_linear: unknown dtype %d", xdtype);
   hipStream_t st = (hipStream_t)stream;
+  const int KT = (int)ceil_div(k, 128), KG = (int)ceil_div(k, 512), K = (int)k;
+  const int64_t ntn = ceil_div(N, 16), mtn = ceil_div(M, 16);
+  const size_t lds = (size_t)KT * 1024 + (size_t)KG * 256;       // x in 4 bits
+  if (mtn == 1 && lds <= 64 * 1024) {
+    by_dtype(xdtype, "", [&](auto* xtag) {
+      by_dtype(ydtype, "", [&](auto* ytag) {
+        using TX = std::remove_pointer_t<decltype(xtag)>;
+        using T = std::remove_pointer_t<decltype(ytag)>;
+        hipLaunchKernelGGL((mxfp4_linear_rows_kernel<TX, T>), dim3((unsigned)ceil_div(ntn, 4)), dim3(256), lds, st, (const TX*)x, ldx, (int)M, (const uint4*)wcodes,
+                           (const unsigned int*)wscales, (int)N, K, KT, KG, bias, (T*)y, ldy);
+      });
+    });
+    LEC_CHECK_LAUNCH("mxfp4_linear_rows_kernel");
+    return LEC_OK;
+  }
   void* xs = (char*)workspace + codes_bytes(M, k);
-  const int rc = quantize(x, xdtype, ldx, M, (int)k, workspace, xs, st);
+  const int rc = quantize(x, xdtype, ldx, M, K, workspace, xs, st);
   if (rc != LEC_OK) return rc;
-  const int KT = (int)ceil_div(k, 128), KG = (int)ceil_div(k, 512);
-  const int64_t gy = ceil_div(M, 128);
-  LEC_CHECK_ARG(gy <= 65535, "mxfp4_linear: %lld rows in one call (at most %d)", (long long)M, 65535 * 128);
-  by_dtype(ydtype, "mxfp4_linear", [&](auto* tag) {
+  const int64_t nbn = ceil_div(N, 256), nbm = ceil_div(M, 256);
+  if (nbn * nbm >= 128 && KT <= 32768) {
+    const int64_t per = ceil_div(nbn * nbm, 8);
+    LEC_CHECK_ARG(per <= (1 << 20), "mxfp4_linear: y has %lld tiles, too many for one call", (long long)(nbn * nbm));
+    int rl = LEC_OK;
+    by_dtype(ydtype, "", [&](auto* tag) {
+      using T = std::remove_pointer_t<decltype(tag)>;
+      static const hipError_t set = hipFuncSetAttribute((const void*)mxfp4_linear_big_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+      if (set != hipSuccess) { rl = hip_fail(set, "mxfp4_linear_big_kernel"); return; }
+      hipLaunchKernelGGL((mxfp4_linear_big_kernel<T>), dim3((unsigned)(per * 8)), dim3(256), 128 * 1024, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
+                         (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy, (int)nbn, (int)nbm, (int)per);
+    });
+    if (rl != LEC_OK) return rl;
+    LEC_CHECK_LAUNCH("mxfp4_linear_big_kernel");
+    return LEC_OK;
+  }
+  int rl = LEC_OK;
+  by_dtype(ydtype, "", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    hipLaunchKernelGGL((mxfp4_linear_kernel<T, 4, 4>), dim3((unsigned)ceil_div(N, 128), (unsigned)gy), dim3(256), 0, st, (const uint4*)workspace, (const unsigned int*)xs, M,
-                       (const uint4*)wcodes, (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy);
+    auto run = [&](auto kernel, int WN, int WM, int NT, int MT) {
+      const int64_t gy = ceil_div(mtn, WM * MT);
+      if (gy > 65535) { set_error("mxfp4_linear: %lld rows in one call of %lld classes, too many", (long long)M, (long long)N); rl = LEC_E_ARG; return; }
+      hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(ntn, WN * NT), (unsigned)gy), dim3(64 * WN * WM), 0, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
+                         (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy);
+    };
+    if (mtn <= 4) run(mxfp4_linear_small_kernel<T, 4, 1, 1, 4>, 4, 1, 1, 4);
+    else if (ntn * mtn <= 4096) run(mxfp4_linear_small_kernel<T, 2, 2, 1, 2>, 2, 2, 1, 2);
+    else run(mxfp4_linear_small_kernel<T, 2, 2, 4, 4>, 2, 2, 4, 4);
   });
-  LEC_CHECK_LAUNCH("mxfp4_linear_kernel");
+  if (rl != LEC_OK) return rl;
+  LEC_CHECK_LAUNCH("mxfp4_linear_small_kernel");
   return LEC_OK;
 }

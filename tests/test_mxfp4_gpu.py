@@ -111,6 +111,17 @@ def test_large_heads(M, N):
     check(quant.MXFP4Linear(w.cuda(), b.cuda())(x.cuda()), x, w, b, 'bf16')
 
 
+@pytest.mark.parametrize('M,N,K,dtype,out', [(2300, 5003, 640, 'bf16', 'bf16'), (4096, 2048, 512, 'fp32', 'fp32'), (2049, 4100, 130, 'fp16', 'fp16'), (300, 17000, 1300, 'bf16', 'fp32'),
+                                               (9000, 1001, 33, 'bf16', 'bf16'), (2561, 3001, 2048, 'bf16', 'bf16')])
+def test_products_large_enough_for_the_ring(M, N, K, dtype, out):
+    from learning_embeddings_amd import quant
+    x, w, b = head(M, N, K, dtype, out, True, seed=5)
+    h = quant.MXFP4Linear(w.cuda(), b.cuda(), out_dtype=DT[out])
+    y = h(x.cuda())
+    check(y, x, w, b, out)
+    assert torch.equal(y, h(x.cuda())) and torch.equal(y[:77], h(x.cuda()[:77]))
+
+
 @pytest.mark.parametrize('M', [1, 20, 300])
 def test_blocks_without_a_value_poison_their_row_and_column_only(M):
     from learning_embeddings_amd import quant
