@@ -286,9 +286,9 @@ int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t R, in
  * (6c) Microscaled 4-bit floating point (MXFP4): quantisation, its inverse, the product of a frozen classifier head.  No counterpart in the reference.
  *      Blocks of 32 elements along a row share X = 2^clamp(floor(log2 max|v|) - 2, -127, 127), kept as the byte log2 X + 127; an element is v / X rounded to
  *      nearest (ties to even) into {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign, saturating.  A block with a NaN or an infinity: byte 255, stands for NaN.
- *      codes:  [ceil(rows / 16)][ceil(k / 128)][64 lanes][16 bytes]: lane l holds row l % 16, elements 32 (l / 16) .. + 32 of the tile, low nibble first
- *      scales: [ceil(rows / 16)][ceil(k / 512)][64 lanes][4 bytes]:  lane l's scale bytes of four consecutive 128-element tiles
- *      Padding is zero.  Both 16-byte aligned, lec_mxfp4_{codes,scales}_bytes() long (negative: bad sizes; rows <= 2^31 - 16, k <= 2^24).
+ *      codes:  [ceil(rows / 32)][ceil(k / 64)][64 lanes][16 bytes]: lane l holds row l % 32, elements 32 (l / 32) .. + 32 of the tile, low nibble first
+ *      scales: [ceil(rows / 32)][ceil(k / 256)][64 lanes][4 bytes]: lane l's scale bytes of four consecutive 64-element tiles
+ *      Padding is zero.  Both 16-byte aligned, lec_mxfp4_{codes,scales}_bytes() long (negative: bad sizes; rows <= 2^31 - 32, k <= 2^24).
  *      x: [rows, k] of `dtype`, row stride ld >= k, element-aligned.  dequantize writes fp32 or bf16 (both exact).
  *      linear: y[M, N] (ydtype, ldy) = x_4 w_4^T + bias; x is quantised by the call into `workspace` (lec_mxfp4_linear_workspace_bytes, one call in flight per
  *      workspace), products are exact, sums 32-bit in a fixed order, bias (fp32 [N] or NULL) is added in 32 bits, one rounding to ydtype.

@@ -4,10 +4,12 @@
 // log2 X + 127; an element is v / X rounded to nearest, ties to even, into {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign, saturating at 6.  A block that holds a NaN or an
 // infinity has the byte 255 and stands for NaN.  17/32 bytes an element.
 //
-// Layout: the matrix instruction's own.  v_mfma_scale_f32_16x16x128_f8f6f4 takes from lane l the 32 codes (16 bytes) of row l % 16, elements 32 (l / 16) .. + 32 of a
-// 128-element stretch, and one scale byte for them.  So a tile of 16 rows x 128 elements is 1 KB in lane order (codes[row tile][k tile][lane][16]): a wave's operand
-// load is one contiguous 1 KB, from memory or from LDS, with no bank conflict and no shuffle.  The scale bytes of four consecutive k tiles sit in one 32-bit word a
-// lane (scales[row tile][k tile / 4][lane][4]), which the instruction selects a byte of.  Rows are padded to 16 and elements to 128 with zeros.
+// Layout: the matrix instruction's own.  v_mfma_scale_f32_32x32x64_f8f6f4 takes from lane l the 32 codes (16 bytes) of row l % 32, elements 32 (l / 32) .. + 32 of a
+// 64-element stretch, and one scale byte for them.  So a tile of 32 rows x 64 elements is 1 KB in lane order (codes[row tile][k tile][lane][16]): a wave's operand load is
+// one contiguous kilobyte, from memory or from LDS, with no bank conflict and no shuffle.  The scale bytes of four consecutive k tiles sit in one 32-bit word a lane
+// (scales[row tile][k tile / 4][lane][4]), which the instruction selects a byte of.  Rows are padded to 32 and elements to 64 with zeros.
+// (The 16x16x128 form does the same work per instruction in half the cycles, but its issue -- two words for the scales, two for the product -- then takes longer than the
+// product: measured alone 5.4 PFLOP/s with one wave a SIMD and 6.7 with two, against 9.2 and 9.3 for 32x32x64.)
 #include "lec_common.h"
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
@@ -16,10 +18,11 @@ namespace lec {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-static int64_t codes_bytes(int64_t rows, int64_t k) { return ceil_div(rows, 16) * ceil_div(k, 128) * 1024; }
-static int64_t scales_bytes(int64_t rows, int64_t k) { return ceil_div(rows, 16) * ceil_div(k, 512) * 256; }
+static int64_t codes_bytes(int64_t rows, int64_t k) { return ceil_div(rows, 32) * ceil_div(k, 64) * 1024; }
+static int64_t scales_bytes(int64_t rows, int64_t k) { return ceil_div(rows, 32) * ceil_div(k, 256) * 256; }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__hip_bfloat16 v) { return __uint_as_float((unsigned int)*(const unsigned short*)&v << 16); }
@@ -62,30 +65,30 @@ __device__ __forceinline__ unsigned int quantize8(const float (&v)[8], unsigned 
   return e == 255 ? 0u : w;
 }
 
-// A block takes a row tile and a group of four k tiles (16 rows x 512 elements, one scale word a lane of the layout); a wave reads 512 consecutive elements of a row at
-// a time, 16 bytes a lane, so memory sees contiguous kilobytes; the codes of 16 rows meet in the L2.
+// A block takes a row tile and a group of four k tiles (32 rows x 256 elements, one scale word a lane of the layout); half a wave reads 256 consecutive elements of a row,
+// 16 bytes a lane (32 of fp32), so memory sees contiguous runs; the codes of the rows meet in the L2.
 template <typename T>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int K, int KT, int KG, int64_t ntask, unsigned int* __restrict__ codes,
                                                              unsigned int* __restrict__ scales) {
   __shared__ unsigned char s_scale[256];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int ktl = lane >> 4, kb = (lane >> 2) & 3, sub = lane & 3;
+  const int t = threadIdx.x, c = t & 31, r0 = t >> 5;            // eight half waves, four rows each
+  const int ktl = c >> 3, kh = (c >> 2) & 1, sub = c & 3;
   for (int64_t task = blockIdx.x; task < ntask; task += gridDim.x) {
     const int64_t rt = task / KG;
-    const int kg = (int)(task - rt * KG), k = kg * 512 + lane * 8, kt = kg * 4 + ktl;
+    const int kg = (int)(task - rt * KG), k = kg * 256 + c * 8, kt = kg * 4 + ktl;
     float v[4][8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t row = rt * 16 + wave * 4 + i;
+      const int64_t row = rt * 32 + r0 + 8 * i;
       load8(x + row * ld + k, row < rows ? K - k : 0, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = wave * 4 + i;
+      const int r = r0 + 8 * i;
       unsigned int sc;
       const unsigned int w = quantize8(v[i], sc);
-      if (kt < KT) codes[((rt * KT + kt) * 64 + kb * 16 + r) * 4 + sub] = w;
-      if (sub == 0) s_scale[(kb * 16 + r) * 4 + ktl] = (unsigned char)sc;
+      if (kt < KT) codes[((rt * KT + kt) * 64 + kh * 32 + r) * 4 + sub] = w;
+      if (sub == 0) s_scale[(kh * 32 + r) * 4 + ktl] = (unsigned char)sc;
     }
     __syncthreads();
     if (t < 64) scales[(rt * KG + kg) * 64 + t] = ((const unsigned int*)s_scale)[t];
@@ -98,22 +101,22 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <typename T>
 __global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const unsigned int* __restrict__ codes, const unsigned char* __restrict__ scales, int64_t rows, int K, int KT, int KG,
                                                                int64_t ntask, T* __restrict__ out, int64_t ld) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int ktl = lane >> 4, kb = (lane >> 2) & 3, sub = lane & 3;
+  const int t = threadIdx.x, c = t & 31, r0 = t >> 5;
+  const int ktl = c >> 3, kh = (c >> 2) & 1, sub = c & 3;
   for (int64_t task = blockIdx.x; task < ntask; task += gridDim.x) {
     const int64_t rt = task / KG;
-    const int kg = (int)(task - rt * KG), k = kg * 512 + lane * 8, kt = kg * 4 + ktl;
+    const int kg = (int)(task - rt * KG), k = kg * 256 + c * 8, kt = kg * 4 + ktl;
     if (k >= K) continue;
     unsigned int w[4], sc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = wave * 4 + i;                                // (rows past the end are padding of the same tile)
-      w[i] = codes[((rt * KT + kt) * 64 + kb * 16 + r) * 4 + sub];
-      sc[i] = scales[((rt * KG + kg) * 64 + kb * 16 + r) * 4 + ktl];
+      const int r = r0 + 8 * i;                                  // (rows past the end are padding of the same tile)
+      w[i] = codes[((rt * KT + kt) * 64 + kh * 32 + r) * 4 + sub];
+      sc[i] = scales[((rt * KG + kg) * 64 + kh * 32 + r) * 4 + ktl];
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t row = rt * 16 + wave * 4 + i;
+      const int64_t row = rt * 32 + r0 + 8 * i;
       if (row >= rows) continue;
       const float X = sc[i] == 255u ? __builtin_nanf("") : (sc[i] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(sc[i] << 23));      // 2^(byte - 127); byte 0: subnormal
       T v[8];
@@ -133,23 +136,25 @@ __global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const unsigned in
   }
 }
 
-__device__ __forceinline__ f32x4 mfma4(const uint4& a, const uint4& b, f32x4 c, int which, unsigned int sa, unsigned int sb) {
+__device__ __forceinline__ f32x16 mfma4(const uint4& a, const uint4& b, f32x16 c, int which, unsigned int sa, unsigned int sb) {
   i32x8 av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
   switch (which) {                                               // (the selected byte is part of the instruction)
-    case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
-    case 1: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 1, (int)sa, 1, (int)sb);
-    case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 2, (int)sa, 2, (int)sb);
-    default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 3, (int)sa, 3, (int)sb);
+    case 0: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
+    case 1: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 1, (int)sa, 1, (int)sb);
+    case 2: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 2, (int)sa, 2, (int)sb);
+    default: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 3, (int)sa, 3, (int)sb);
   }
 }
+__device__ __forceinline__ f32x16 zero16() { return f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
 
-// y[m, n] = sum_k x[m, k] w[n, k] + bias[n].  The weights are the A operand: a lane's four accumulators are four consecutive classes n of one row m.
+// y[m, n] = sum_k x[m, k] w[n, k] + bias[n].  The weights are the A operand: of a tile of 32 classes x 32 rows a lane holds row m = lane % 32 and, in registers
+// 4 g .. 4 g + 3, the classes 8 g + 4 (lane / 32) .. + 4.
 template <typename T>
-__device__ __forceinline__ void store4(T* __restrict__ y, int64_t ldy, int64_t M, int N, int64_t m, int n, const f32x4& acc, const float (&bv)[4]) {
+__device__ __forceinline__ void store4(T* __restrict__ y, int64_t ldy, int64_t M, int N, int64_t m, int n, const float (&v)[4]) {
   if (m >= M || n >= N) return;
   T o[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(acc[e] + bv[e]);
+  for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(v[e]);
   T* p = y + m * ldy + n;
   if (n + 4 <= N) __builtin_memcpy((void*)p, o, sizeof(o));
   else {
@@ -157,63 +162,77 @@ __device__ __forceinline__ void store4(T* __restrict__ y, int64_t ldy, int64_t M
     for (int e = 0; e < 4; ++e) if (n + e < N) p[e] = o[e];
   }
 }
-__device__ __forceinline__ void load_bias(const float* __restrict__ bias, int N, int n, float (&bv)[4]) {
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t make_rsrc(const void* p, unsigned bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00020000); }
+__device__ __forceinline__ float bias_at(const rsrc_t& r, int n) { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, n * 4, 0, 0)); }      // past the end, or no bias: 0
+
+template <typename T>
+__device__ __forceinline__ void store_tile(T* __restrict__ y, int64_t ldy, int64_t M, int N, int64_t m0, int n0, int lane, const rsrc_t& rbias, const f32x16& acc) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) bv[e] = bias && n + e < N ? bias[n + e] : 0.0f;
+  for (int g = 0; g < 4; ++g) {
+    const int n = n0 + 8 * g + 4 * (lane >> 5);
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = acc[4 * g + e] + bias_at(rbias, n + e);
+    store4(y, ldy, M, N, m0 + (lane & 31), n, v);
+  }
 }
 
-// At most 16 rows (one tile of x): the time is the weights' way from memory.  A wave owns one tile of 16 classes and asks for 16 k tiles of its weights at once; while
-// they are under way the block quantises x into LDS (each block again: x is small and comes from the L2, a launch of its own would cost more).  x has to fit 64 KB of LDS: K <= 7680.
+// At most 32 rows (one tile of x): the time is the weights' way from memory.  Two waves share a tile of 32 classes, each half of its k tiles (of a chunk of 32), all asked for
+// at once; while they are under way the block quantises x into LDS (each block again: x is small and comes from the L2, a launch of its own would cost more).  x has to fit
+// LDS beside the join: K <= 3 328.  Columns of x's tile that are no row of x are never written: a column of the product depends on its own column only, and those are not stored.
 template <typename TX, typename T>
 __global__ __launch_bounds__(256) void mxfp4_linear_rows_kernel(const TX* __restrict__ x, int64_t ldx, int M, const uint4* __restrict__ wc, const unsigned int* __restrict__ wsc, int N, int K,
                                                                 int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   unsigned int* xcodes = (unsigned int*)smem;                    // [KT][64][4] words
   unsigned char* xscale = smem + (size_t)KT * 1024;              // [KG][64][4] bytes
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int nt = min((int)blockIdx.x * 4 + wave, ((N + 15) >> 4) - 1);
-  const bool mine = (int)blockIdx.x * 4 + wave == nt;            // (a wave past the last tile repeats it and stores nothing)
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = wave & 1;
+  const int ntn = (N + 31) >> 5, nt_ = (int)blockIdx.x * 2 + (wave >> 1), nt = min(nt_, ntn - 1);        // (a pair past the last tile repeats it and stores nothing)
   constexpr int CH = 16;
   uint4 w[CH];
   unsigned int sw[CH / 4];
-  auto fetch = [&](int kt0) {
+  auto fetch = [&](int kt0) {                                    // this wave's tiles of the chunk: kt0 + 16 half .. + 16
 #pragma unroll
-    for (int i = 0; i < CH; ++i) if (kt0 + i < KT) w[i] = wc[((int64_t)nt * KT + kt0 + i) * 64 + lane];
+    for (int i = 0; i < CH; ++i) if (kt0 + CH * half + i < KT) w[i] = wc[((int64_t)nt * KT + kt0 + CH * half + i) * 64 + lane];
 #pragma unroll
-    for (int i = 0; i < CH / 4; ++i) if (kt0 / 4 + i < KG) sw[i] = wsc[((int64_t)nt * KG + kt0 / 4 + i) * 64 + lane];
+    for (int i = 0; i < CH / 4; ++i) if (kt0 / 4 + CH / 4 * half + i < KG) sw[i] = wsc[((int64_t)nt * KG + kt0 / 4 + CH / 4 * half + i) * 64 + lane];
   };
   fetch(0);
-  for (int i = t; i < KT * 64; i += 256) ((uint4*)xcodes)[i] = make_uint4(0u, 0u, 0u, 0u);       // rows that do not exist
-  for (int i = t; i < KG * 64; i += 256) ((unsigned int*)xscale)[i] = 0u;
-  __syncthreads();
-  const int per_row = KG * 64;                                   // 8-element pieces of a row, padded to whole groups of 512
+  const int per_row = KG * 32;                                   // 8-element pieces of a row, padded to whole groups of 256
   for (int i = t; i < M * per_row; i += 256) {
-    const int r = i / per_row, q = i - r * per_row, k = q * 8, kt = k >> 7, kb = (k >> 5) & 3, sub = (k >> 3) & 3;
+    const int r = i / per_row, q = i - r * per_row, k = q * 8, kt = k >> 6, kh = (k >> 5) & 1, sub = (k >> 3) & 3;
     float v[8];
     load8(x + (int64_t)r * ldx + k, K - k, v);
     unsigned int sc;
     const unsigned int c = quantize8(v, sc);
-    if (kt < KT) xcodes[(kt * 64 + kb * 16 + r) * 4 + sub] = c;
-    if (sub == 0) xscale[((kt >> 2) * 64 + kb * 16 + r) * 4 + (kt & 3)] = (unsigned char)sc;
+    if (kt < KT) xcodes[(kt * 64 + kh * 32 + r) * 4 + sub] = c;
+    if (sub == 0) xscale[((kt >> 2) * 64 + kh * 32 + r) * 4 + (kt & 3)] = (unsigned char)sc;
   }
   __syncthreads();
-  f32x4 acc[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};                // two chains: an MFMA need not wait for the one before
-  for (int kt0 = 0; kt0 < KT; kt0 += CH) {
+  f32x16 acc = zero16();
+  for (int kt0 = 0; kt0 < KT; kt0 += 2 * CH) {
     if (kt0) fetch(kt0);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      if (kt0 + i < KT) {
-        const uint4 b = ((const uint4*)xcodes)[(kt0 + i) * 64 + lane];
-        const unsigned int sb = ((const unsigned int*)xscale)[((kt0 + i) >> 2) * 64 + lane];
-        acc[i & 1] = mfma4(w[i], b, acc[i & 1], i & 3, sw[i >> 2], sb);
-      }
+      const int kt = kt0 + CH * half + i;
+      if (kt < KT) acc = mfma4(w[i], ((const uint4*)xcodes)[kt * 64 + lane], acc, i & 3, sw[i >> 2], ((const unsigned int*)xscale)[(kt >> 2) * 64 + lane]);
     }
   }
-  if (!mine) return;
-  const int n = nt * 16 + 4 * (lane >> 4);
-  float bv[4];
-  load_bias(bias, N, n, bv);
-  store4(y, ldy, M, N, lane & 15, n, acc[0] + acc[1], bv);
+  __shared__ f32x4 s_half[2][4][64];                             // the second half's sums, joined in a fixed order
+  if (half) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) s_half[wave >> 1][g][lane] = f32x4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+  }
+  __syncthreads();
+  if (half || nt_ != nt) return;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 o = s_half[wave >> 1][g][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[4 * g + e] += o[e];
+  }
+  store_tile(y, ldy, M, N, 0, nt * 32, lane, make_rsrc(bias, bias ? (unsigned)N * 4u : 0u), acc);
 }
 
 // A block of WN x WM waves, a wave NT x MT tiles, operands straight from memory (every load is a contiguous kilobyte): few tiles, or shapes too small for the ring below.
@@ -222,14 +241,14 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_linear_small_kernel(const 
                                                                           const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y,
                                                                           int64_t ldy) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nt0 = ((int)blockIdx.x * WN + wave % WN) * NT, ntn = (N + 15) >> 4;
-  const int64_t mt0 = ((int64_t)blockIdx.y * WM + wave / WN) * MT, mtn = (M + 15) >> 4;
+  const int nt0 = ((int)blockIdx.x * WN + wave % WN) * NT, ntn = (N + 31) >> 5;
+  const int64_t mt0 = ((int64_t)blockIdx.y * WM + wave / WN) * MT, mtn = (M + 31) >> 5;
   if (nt0 >= ntn || mt0 >= mtn) return;
-  f32x4 acc[NT][MT];
+  f32x16 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < MT; ++j) acc[i][j] = zero16();
   for (int kg = 0; kg < KG; ++kg) {
     unsigned int sa[NT], sb[MT];
 #pragma unroll
@@ -251,22 +270,18 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_linear_small_kernel(const 
         for (int j = 0; j < MT; ++j) acc[i][j] = mfma4(a[i], b[j], acc[i][j], q, sa[i], sb[j]);
     }
   }
+  const rsrc_t rbias = make_rsrc(bias, bias ? (unsigned)N * 4u : 0u);
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int n = (nt0 + i) * 16 + 4 * (lane >> 4);
-    float bv[4];
-    load_bias(bias, N, n, bv);
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) store4(y, ldy, M, N, (mt0 + j) * 16 + (lane & 15), n, acc[i][j], bv);
-  }
+    for (int j = 0; j < MT; ++j) store_tile(y, ldy, M, N, (mt0 + j) * 32, (nt0 + i) * 32, lane, rbias, acc[i][j]);
 }
 
-// Large products.  A block of 2 x 2 waves owns 256 x 256 of y, a wave 128 x 128 (8 x 8 tiles, 256 accumulators: one wave a SIMD, one block a CU).  A k tile of both operands is
-// 32 KB; a ring of four stages in LDS is filled by LDS-DMA (a wave's request is one contiguous kilobyte = one operand tile in lane order, so there is nothing to swizzle), three stages
-// ahead.  Per k tile a wave issues 64 MFMAs of 16 cycles and reads 16 KB of LDS: 96 KB of LDS traffic per 1024 cycles a CU, under its 128 B / clk.
+// Large products.  A block of 2 x 2 waves owns 256 x 256 of y, a wave 128 x 128 (4 x 4 tiles, 256 accumulators: one wave a SIMD, one block a CU).  A stage of the ring is two k
+// tiles (128 elements) of both operands, 32 KB; four stages in LDS are filled by LDS-DMA (a wave's request is one contiguous kilobyte = one operand tile in lane order, so there
+// is nothing to swizzle), three stages ahead.  Per stage a wave issues 32 MFMAs of 32 cycles and reads 16 KB of LDS: 96 KB of LDS traffic per 1024 cycles a CU, under its
+// 128 B / clk.
 typedef __attribute__((address_space(3))) void lds_ptr;
-typedef __amdgpu_buffer_rsrc_t rsrc_t;
-__device__ __forceinline__ rsrc_t make_rsrc(const void* p, unsigned bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00020000); }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); __builtin_amdgcn_s_barrier(); asm volatile("" ::: "memory"); }
 
@@ -274,11 +289,11 @@ __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)" :::
 // LDS-DMA before any read of LDS -- the ring would be one stage deep.)
 template <typename T>
 __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
-                                                                  const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy,
-                                                                  int nbn, int nbm, int per_xcd) {
+                                                      const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy, int nbn,
+                                                      int nbm, int per_xcd) {
   constexpr int STAGE = 32 * 1024, IPW = 8;                      // bytes of a stage; LDS-DMA instructions a wave issues for one
   constexpr int PIN = (int)0x80000000;                           // a volatile load: it stays where it is written, ahead of the requests behind it
-  constexpr int OOB = 0x40000000;                                // past any operand buffer (KT <= 32 768: at most 2^29 bytes)
+  constexpr int OOB = 0x40000000;                                // past any operand buffer (KT <= 32 768: at most 2^28 bytes)
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave & 1, wm = wave >> 1;
@@ -288,112 +303,128 @@ __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ 
   if (g >= (int64_t)nbn * nbm) return;
   const int band = (int)(g / (4 * (int64_t)nbn)), inb = (int)(g - (int64_t)band * 4 * nbn), bw = min(4, nbm - band * 4);
   const int bn = __builtin_amdgcn_readfirstlane(inb / bw), bm = __builtin_amdgcn_readfirstlane(band * 4 + inb % bw);      // (the division leaves them in vector registers)
-  const int ntn = (N + 15) >> 4, mtn = (int)((M + 15) >> 4);
+  const int ntn = (N + 31) >> 5, mtn = (int)((M + 31) >> 5);
   // The block's operand tiles of each side and their scales as buffers that end with the last of them; a tile past the matrix repeats the last one (and is not stored).
-  const int na_ = min(16, ntn - bn * 16), nb_ = min(16, mtn - bm * 16);
-  const rsrc_t ra = make_rsrc(wc + (int64_t)bn * 16 * KT * 64, (unsigned)na_ * KT * 1024), rb = make_rsrc(xc + (int64_t)bm * 16 * KT * 64, (unsigned)nb_ * KT * 1024);
-  const rsrc_t rsa = make_rsrc(wsc + (int64_t)bn * 16 * KG * 64, (unsigned)na_ * KG * 256), rsb = make_rsrc(xs + (int64_t)bm * 16 * KG * 64, (unsigned)nb_ * KG * 256);
-  auto issue = [&](int kt) {                                     // this wave's tiles of stage kt: 4 of the weights, 4 of x.  Past the last stage: no traffic, zeros in LDS
-    unsigned char* base = smem + (kt & 3) * STAGE + wave * 1024;
-    const int voff = lane * 16 + (kt < KT ? 0 : OOB), kc = min(kt, KT - 1);
+  const int na_ = min(8, ntn - bn * 8), nb_ = min(8, mtn - bm * 8);
+  const rsrc_t ra = make_rsrc(wc + (int64_t)bn * 8 * KT * 64, (unsigned)na_ * KT * 1024), rb = make_rsrc(xc + (int64_t)bm * 8 * KT * 64, (unsigned)nb_ * KT * 1024);
+  const rsrc_t rsa = make_rsrc(wsc + (int64_t)bn * 8 * KG * 64, (unsigned)na_ * KG * 256), rsb = make_rsrc(xs + (int64_t)bm * 8 * KG * 64, (unsigned)nb_ * KG * 256);
+  // Stage st: [weights: 8 row tiles x 2 k tiles | x: the same], a kilobyte each.  Wave w takes k tile w % 2 of the row tiles w / 2 + 2 u.  Past the last k tile: no traffic,
+  // zeros in LDS.
+  auto issue = [&](int st) {
+    unsigned char* base = smem + (st & 3) * STAGE + wave * 1024;
+    const int kt = 2 * st + (wave & 1), kc = min(kt, KT - 1), voff = lane * 16 + (kt < KT ? 0 : OOB);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr*)(base + u * 4096), 16, voff, (min(wave + 4 * u, na_ - 1) * KT + kc) * 1024, 0, 0);
+    for (int u = 0; u < 4; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr*)(base + u * 4096), 16, voff, (min((wave >> 1) + 2 * u, na_ - 1) * KT + kc) * 1024, 0, 0);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr*)(base + 16384 + u * 4096), 16, voff, (min(wave + 4 * u, nb_ - 1) * KT + kc) * 1024, 0, 0);
+    for (int u = 0; u < 4; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr*)(base + 16384 + u * 4096), 16, voff, (min((wave >> 1) + 2 * u, nb_ - 1) * KT + kc) * 1024, 0, 0);
   };
-  f32x4 acc[8][8];
+  f32x16 acc[4][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  int sa[8], sb[8], na[8], nb[8];                                // scale words: of this group of four k tiles, of the next one
+    for (int j = 0; j < 4; ++j) acc[i][j] = zero16();
+  int sa[4], sb[4], na[4], nb[4];                                // scale words: of this group of four k tiles, of the next one
   auto fetch_scales = [&](int kg) {                              // (a group past the end: the last one again)
     const int kc = min(kg, KG - 1);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      na[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, lane * 4, (min(wn * 8 + i, na_ - 1) * KG + kc) * 256, PIN);
-      nb[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, lane * 4, (min(wm * 8 + i, nb_ - 1) * KG + kc) * 256, PIN);
+    for (int i = 0; i < 4; ++i) {
+      na[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, lane * 4, (min(wn * 4 + i, na_ - 1) * KG + kc) * 256, PIN);
+      nb[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, lane * 4, (min(wm * 4 + i, nb_ - 1) * KG + kc) * 256, PIN);
     }
   };
-  const uint4* A = (const uint4*)smem + wn * 512 + lane;         // this wave's operand tiles of slot 0
+  const uint4* A = (const uint4*)smem + wn * 512 + lane;         // this wave's operand tiles of slot 0: [4 row tiles][2 k tiles]
   const uint4* B = (const uint4*)(smem + 16384) + wm * 512 + lane;
   fetch_scales(0);
   issue(0); issue(1); issue(2); issue(3);
   wait_vm<3 * IPW>();                                            // stage 0 has landed for this wave ...
   meet();                                                        // ... and for every wave
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     sa[i] = na[i]; sb[i] = nb[i];
     asm volatile("" : "+v"(sa[i]), "+v"(sb[i]));                  // in registers before the loop: its own waits then count the loop's requests only
   }
-  uint4 a = A[0], b[8];
+  uint4 a = A[0], b[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) b[j] = B[j * 64];
-  // One k tile: rows 0 .. 3 of the products run while the wave reads its other weights of the stage; then everybody is done reading stage kt, whose slot takes stage kt + 4, and
-  // stage kt + 1 has landed once at most the two younger stages' requests are outstanding (scale loads in between only make the wait stricter); rows 4 .. 7 run while
-  // stage kt + 1's first operands are read.  The order is pinned: left alone the scheduler puts every read before the first product.  Groups of four k tiles, the last one
-  // filled up with stages of zeros, so that the body has no branch.
-  auto tile = [&](int kt, auto qc) {
+  for (int j = 0; j < 4; ++j) b[j] = B[j * 128];
+  // One stage: its first k tile's products run while the wave reads the rest of the stage; then everybody is done reading stage st, whose slot takes stage st + 4, and stage
+  // st + 1 has landed once at most the two younger stages' requests are outstanding (scale loads in between only make the wait stricter); the second k tile's products run while
+  // stage st + 1's first operands are read.  The order is pinned: left alone the scheduler puts every read before the first product.  Groups of two stages, the last one filled
+  // up with zeros, so that the body has no branch.
+  auto stage = [&](int st, auto qc) {
     constexpr int q = decltype(qc)::value;
-    const uint4* Ao = A + q * (STAGE / 16);
-    const uint4* An = A + ((q + 1) & 3) * (STAGE / 16);
-    const uint4* Bn = B + ((q + 1) & 3) * (STAGE / 16);
-    uint4 ar[8], bx[8];
-    ar[0] = a;
+    const int o = (st & 3) * (STAGE / 16), on = ((st + 1) & 3) * (STAGE / 16);
+    uint4 a0[4], a1[4], b1[4], bx[4];
+    a0[0] = a;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      ar[i + 1] = Ao[(i + 1) * 64];
-      if (i > 0) ar[i + 4] = Ao[(i + 4) * 64];
+      if (i < 3) a0[i + 1] = A[o + (i + 1) * 128];
+      b1[i] = B[o + i * 128 + 64];
+      a1[i] = A[o + i * 128 + 64];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[i][j] = mfma4(ar[i], b[j], acc[i][j], q, sa[i], sb[j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma4(a0[i], b[j], acc[i][j], q, sa[i], sb[j]);
       __builtin_amdgcn_sched_barrier(0);
     }
     wait_vm<2 * IPW>();
     meet();
-    if (q == 0) fetch_scales((kt >> 2) + 1);
-    issue(kt + 4);
+    if (q == 0) fetch_scales((st >> 1) + 1);
+    issue(st + 4);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 4; i < 8; ++i) {
-      if (i == 4) a = An[0];
-      bx[2 * (i - 4)] = Bn[2 * (i - 4) * 64];
-      bx[2 * (i - 4) + 1] = Bn[(2 * (i - 4) + 1) * 64];
+    for (int i = 0; i < 4; ++i) {
+      if (i == 0) a = A[on];
+      bx[i] = B[on + i * 128];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[i][j] = mfma4(ar[i], b[j], acc[i][j], q, sa[i], sb[j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma4(a1[i], b1[j], acc[i][j], q + 1, sa[i], sb[j]);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = bx[j];
+    for (int j = 0; j < 4; ++j) b[j] = bx[j];
   };
-  for (int kt = 0; kt < KT; kt += 4) {
-    tile(kt, std::integral_constant<int, 0>{});
-    tile(kt + 1, std::integral_constant<int, 1>{});
-    tile(kt + 2, std::integral_constant<int, 2>{});
-    tile(kt + 3, std::integral_constant<int, 3>{});
+  for (int st = 0; 2 * st < KT; st += 2) {
+    stage(st, std::integral_constant<int, 0>{});
+    stage(st + 1, std::integral_constant<int, 2>{});
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { sa[i] = na[i]; sb[i] = nb[i]; }
+    for (int i = 0; i < 4; ++i) { sa[i] = na[i]; sb[i] = nb[i]; }
   }
   wait_vm<0>();                                                  // (the stages of zeros past the end still write LDS)
   const rsrc_t rbias = make_rsrc(bias, bias ? (unsigned)N * 4u : 0u);
   const bool inside = (bn + 1) * 256 <= N && (int64_t)(bm + 1) * 256 <= M;
+  const int64_t m0 = (int64_t)bm * 256 + wm * 128;
+  const int n0 = bn * 256 + wn * 128;
+  if (inside) {
+    // lanes l and l + 32 hold the two halves of eight classes: one exchange of half waves between two groups of registers gives every lane eight consecutive classes
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int n = (bn * 16 + wn * 8 + i) * 16 + 4 * (lane >> 4);
-    float bv[4];
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bv[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rbias, (n + e) * 4, 0, 0));       // (past the end: 0)
+      for (int h = 0; h < 2; ++h) {
+        float bl[4], bh[4];
+        const int nl = n0 + i * 32 + 16 * h + 4 * (lane >> 5);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t m = (int64_t)(bm * 16 + wm * 8 + j) * 16 + (lane & 15);
-      if (inside) {
-        T o[4];
+        for (int e = 0; e < 4; ++e) { bl[e] = bias_at(rbias, nl + e); bh[e] = bias_at(rbias, nl + 8 + e); }
+        T* p = y + (m0 + (lane & 31)) * ldy + n0 + i * 32 + 16 * h + 8 * (lane >> 5);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(acc[i][j][e] + bv[e]);
-        __builtin_memcpy((void*)(y + m * ldy + n), o, sizeof(o));
-      } else {
-        store4(y, ldy, M, N, m, n, acc[i][j], bv);
+        for (int j = 0; j < 4; ++j) {
+          T o[8];
+          __attribute__((aligned(16))) T lo[4], hi[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { lo[e] = from_f32<T>(acc[i][j][8 * h + e] + bl[e]); hi[e] = from_f32<T>(acc[i][j][8 * h + 4 + e] + bh[e]); }
+          constexpr int W = sizeof(T);                           // words of four elements
+          unsigned int ul[W], uh[W];
+          __builtin_memcpy(ul, lo, sizeof(ul)); __builtin_memcpy(uh, hi, sizeof(uh));
+#pragma unroll
+          for (int k = 0; k < W; ++k) {
+            const auto s = __builtin_amdgcn_permlane32_swap(ul[k], uh[k], false, false);      // (ul low | uh low) , (ul high | uh high) by halves of the wave
+            ul[k] = s[0]; uh[k] = s[1];
+          }
+          __builtin_memcpy(o, ul, sizeof(ul)); __builtin_memcpy(o + 4, uh, sizeof(uh));
+          __builtin_memcpy((void*)(p + (int64_t)j * 32 * ldy), o, sizeof(o));
+        }
       }
-    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) store_tile(y, ldy, M, N, m0 + j * 32, n0 + i * 32, lane, rbias, acc[i][j]);
   }
 }
 
@@ -416,8 +447,8 @@ template <typename F> static int by_dtype(int dtype, const char* what, F&& f) {
 static unsigned grid_of(int64_t blocks) { return (unsigned)(blocks > (1 << 22) ? (1 << 22) : blocks); }
 
 static int quantize(const void* x, int dtype, int64_t ld, int64_t rows, int K, void* codes, void* scales, hipStream_t st) {
-  const int KT = (int)ceil_div(K, 128), KG = (int)ceil_div(K, 512);
-  const int64_t ntask = ceil_div(rows, 16) * KG;
+  const int KT = (int)ceil_div(K, 64), KG = (int)ceil_div(K, 256);
+  const int64_t ntask = ceil_div(rows, 32) * KG;
   const int rc = by_dtype(dtype, "mxfp4_quantize", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     hipLaunchKernelGGL((mxfp4_quantize_kernel<T>), dim3(grid_of(ntask)), dim3(256), 0, st, (const T*)x, ld, rows, K, KT, KG, ntask, (unsigned int*)codes, (unsigned int*)scales);
@@ -429,7 +460,7 @@ static int quantize(const void* x, int dtype, int64_t ld, int64_t rows, int K, v
 
 }  // namespace lec
 
-static bool sizes_ok(int64_t rows, int64_t k) { return rows > 0 && rows <= ((int64_t)1 << 31) - 16 && k > 0 && k <= (1 << 24); }
+static bool sizes_ok(int64_t rows, int64_t k) { return rows > 0 && rows <= ((int64_t)1 << 31) - 32 && k > 0 && k <= (1 << 24); }
 
 extern "C" int64_t lec_mxfp4_codes_bytes(int64_t rows, int64_t k) { return sizes_ok(rows, k) ? lec::codes_bytes(rows, k) : LEC_E_ARG; }
 extern "C" int64_t lec_mxfp4_scales_bytes(int64_t rows, int64_t k) { return sizes_ok(rows, k) ? lec::scales_bytes(rows, k) : LEC_E_ARG; }
@@ -446,8 +477,8 @@ extern "C" int lec_mxfp4_dequantize(const void* codes, const void* scales, int64
   LEC_CHECK_ARG(sizes_ok(rows, k), "mxfp4_dequantize: bad sizes rows=%lld k=%lld", (long long)rows, (long long)k);
   LEC_CHECK_ARG(out && codes && scales && ld >= k, "mxfp4_dequantize: null pointer or ld=%lld < k=%lld", (long long)ld, (long long)k);
   LEC_CHECK_ARG(dtype == LEC_DTYPE_F32 || dtype == LEC_DTYPE_BF16, "mxfp4_dequantize: dtype %d does not hold every value (fp32 or bf16)", dtype);
-  const int KT = (int)ceil_div(k, 128), KG = (int)ceil_div(k, 512);
-  const int64_t ntask = ceil_div(rows, 16) * KG;
+  const int KT = (int)ceil_div(k, 64), KG = (int)ceil_div(k, 256);
+  const int64_t ntask = ceil_div(rows, 32) * KG;
   if (dtype == LEC_DTYPE_F32)
     hipLaunchKernelGGL((mxfp4_dequantize_kernel<float>), dim3(grid_of(ntask)), dim3(256), 0, (hipStream_t)stream, (const unsigned int*)codes, (const unsigned char*)scales, rows, (int)k, KT, KG,
                        ntask, (float*)out, ld);
@@ -472,15 +503,15 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
   LEC_CHECK_ARG(ydtype == LEC_DTYPE_F32 || ydtype == LEC_DTYPE_BF16 || ydtype == LEC_DTYPE_F16, "mxfp4_linear: unknown dtype %d", ydtype);
   LEC_CHECK_ARG(xdtype == LEC_DTYPE_F32 || xdtype == LEC_DTYPE_BF16 || xdtype == LEC_DTYPE_F16, "mxfp4_linear: unknown dtype %d", xdtype);
   hipStream_t st = (hipStream_t)stream;
-  const int KT = (int)ceil_div(k, 128), KG = (int)ceil_div(k, 512), K = (int)k;
-  const int64_t ntn = ceil_div(N, 16), mtn = ceil_div(M, 16);
+  const int KT = (int)ceil_div(k, 64), KG = (int)ceil_div(k, 256), K = (int)k;
+  const int64_t ntn = ceil_div(N, 32), mtn = ceil_div(M, 32);
   const size_t lds = (size_t)KT * 1024 + (size_t)KG * 256;       // x in 4 bits
-  if (mtn == 1 && lds <= 64 * 1024) {
+  if (mtn == 1 && lds <= 64 * 1024 - 8192) {
     by_dtype(xdtype, "", [&](auto* xtag) {
       by_dtype(ydtype, "", [&](auto* ytag) {
         using TX = std::remove_pointer_t<decltype(xtag)>;
         using T = std::remove_pointer_t<decltype(ytag)>;
-        hipLaunchKernelGGL((mxfp4_linear_rows_kernel<TX, T>), dim3((unsigned)ceil_div(ntn, 4)), dim3(256), lds, st, (const TX*)x, ldx, (int)M, (const uint4*)wcodes,
+        hipLaunchKernelGGL((mxfp4_linear_rows_kernel<TX, T>), dim3((unsigned)ceil_div(ntn, 2)), dim3(256), lds, st, (const TX*)x, ldx, (int)M, (const uint4*)wcodes,
                            (const unsigned int*)wscales, (int)N, K, KT, KG, bias, (T*)y, ldy);
       });
     });
@@ -515,9 +546,9 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
       hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(ntn, WN * NT), (unsigned)gy), dim3(64 * WN * WM), 0, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
                          (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy);
     };
-    if (mtn <= 4) run(mxfp4_linear_small_kernel<T, 4, 1, 1, 4>, 4, 1, 1, 4);
-    else if (ntn * mtn <= 4096) run(mxfp4_linear_small_kernel<T, 2, 2, 1, 2>, 2, 2, 1, 2);
-    else run(mxfp4_linear_small_kernel<T, 2, 2, 4, 4>, 2, 2, 4, 4);
+    if (ntn * mtn <= 2048) run(mxfp4_linear_small_kernel<T, 2, 2, 1, 1>, 2, 2, 1, 1);
+    else if (mtn <= 2) run(mxfp4_linear_small_kernel<T, 4, 1, 1, 2>, 4, 1, 1, 2);
+    else run(mxfp4_linear_small_kernel<T, 2, 2, 2, 2>, 2, 2, 2, 2);
   });
   if (rl != LEC_OK) return rl;
   LEC_CHECK_LAUNCH("mxfp4_linear_small_kernel");

@@ -2,7 +2,7 @@
 
 Blocks of 32 elements along a row share a power of two, 2^(floor(log2 max|v|) - 2) within [2^-127, 2^127]; an element is one of
 {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign times it, rounded to nearest with ties to even, saturating.  A block that holds a NaN or an
-infinity stands for NaN.  17/32 bytes an element (rows padded to 16, elements to 128, scale words to 512).
+infinity stands for NaN.  17/32 bytes an element (rows padded to 32, elements to 64, scale words to 256).
 
     head = MXFP4Linear.from_linear(model.fc)          # quantises the weights once
     logits = head(features)                           # quantises the features row by row, multiplies on the 4-bit matrix cores, sums in 32 bits
@@ -74,7 +74,7 @@ def mxfp4_quantize(x):
 
 def _size(n):
     if n < 0:
-        raise ValueError('matrix too large for the 4-bit form (at most 2^31 - 16 rows of 2^24 elements)')
+        raise ValueError('matrix too large for the 4-bit form (at most 2^31 - 32 rows of 2^24 elements)')
     return int(n)
 
 

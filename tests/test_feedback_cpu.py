@@ -181,8 +181,8 @@ def test_mxfp4_refusals():
     with pytest.raises(TypeError, match='exact'):
         quant.MXFP4Tensor(e, e, (0, 32)).dequantize(torch.float16)
     lib = _lib.lib
-    assert lib.lec_mxfp4_codes_bytes(1, 1) == 1024 and lib.lec_mxfp4_codes_bytes(17, 129) == 4096 and lib.lec_mxfp4_scales_bytes(17, 513) == 1024
-    assert lib.lec_mxfp4_codes_bytes(2 ** 31 - 16, 128) == 2 ** 27 * 1024 - 1024 and lib.lec_mxfp4_codes_bytes(0, 1) < 0 and lib.lec_mxfp4_codes_bytes(2 ** 31, 1) < 0
+    assert lib.lec_mxfp4_codes_bytes(1, 1) == 1024 and lib.lec_mxfp4_codes_bytes(33, 65) == 4096 and lib.lec_mxfp4_scales_bytes(33, 257) == 1024
+    assert lib.lec_mxfp4_codes_bytes(2 ** 31 - 32, 64) == 2 ** 26 * 1024 - 1024 and lib.lec_mxfp4_codes_bytes(0, 1) < 0 and lib.lec_mxfp4_codes_bytes(2 ** 31, 1) < 0
     assert lib.lec_mxfp4_codes_bytes(1, 2 ** 24 + 1) < 0 and lib.lec_mxfp4_linear_workspace_bytes(1, 0, 32) < 0
     import ctypes
     p = ctypes.c_void_p(256)
