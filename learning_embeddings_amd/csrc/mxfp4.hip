@@ -65,17 +65,19 @@ __device__ __forceinline__ unsigned int quantize8(const float (&v)[8], unsigned 
   return e == 255 ? 0u : w;
 }
 
-// A block takes a row tile and a group of four k tiles (32 rows x 256 elements, one scale word a lane of the layout); half a wave reads 256 consecutive elements of a row,
-// 16 bytes a lane (32 of fp32), so memory sees contiguous runs; the codes of the rows meet in the L2.
+// A block takes a row tile and a group of four k tiles (32 rows x 256 elements, one scale word a lane of the layout): half a wave reads 256 consecutive elements of a row,
+// 16 bytes a lane (32 of fp32), and the block writes its 4 KB of codes in one piece through LDS (a tile's half is padded by 8 words: the eight halves a wave writes to at
+// once start in different banks).
 template <typename T>
-__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int K, int KT, int KG, int64_t ntask, unsigned int* __restrict__ codes,
+__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int K, int KT, int KG, int64_t ntask, uint4* __restrict__ codes,
                                                              unsigned int* __restrict__ scales) {
+  __shared__ __attribute__((aligned(16))) unsigned int s_code[8 * 136];
   __shared__ unsigned char s_scale[256];
   const int t = threadIdx.x, c = t & 31, r0 = t >> 5;            // eight half waves, four rows each
   const int ktl = c >> 3, kh = (c >> 2) & 1, sub = c & 3;
   for (int64_t task = blockIdx.x; task < ntask; task += gridDim.x) {
     const int64_t rt = task / KG;
-    const int kg = (int)(task - rt * KG), k = kg * 256 + c * 8, kt = kg * 4 + ktl;
+    const int kg = (int)(task - rt * KG), k = kg * 256 + c * 8;
     float v[4][8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -86,13 +88,14 @@ __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict
     for (int i = 0; i < 4; ++i) {
       const int r = r0 + 8 * i;
       unsigned int sc;
-      const unsigned int w = quantize8(v[i], sc);
-      if (kt < KT) codes[((rt * KT + kt) * 64 + kh * 32 + r) * 4 + sub] = w;
+      s_code[(ktl * 2 + kh) * 136 + r * 4 + sub] = quantize8(v[i], sc);
       if (sub == 0) s_scale[(kh * 32 + r) * 4 + ktl] = (unsigned char)sc;
     }
     __syncthreads();
+    const int kt = kg * 4 + (t >> 6);
+    if (kt < KT) codes[(rt * KT + kt) * 64 + (t & 63)] = *(const uint4*)&s_code[(t >> 5) * 136 + (t & 31) * 4];
     if (t < 64) scales[(rt * KG + kg) * 64 + t] = ((const unsigned int*)s_scale)[t];
-    __syncthreads();                                             // (the next task writes s_scale)
+    __syncthreads();                                             // (the next task writes both images)
   }
 }
 
@@ -277,10 +280,17 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_linear_small_kernel(const 
     for (int j = 0; j < MT; ++j) store_tile(y, ldy, M, N, (mt0 + j) * 32, (nt0 + i) * 32, lane, rbias, acc[i][j]);
 }
 
-// Large products.  A block of 2 x 2 waves owns 256 x 256 of y, a wave 128 x 128 (4 x 4 tiles, 256 accumulators: one wave a SIMD, one block a CU).  A stage of the ring is two k
-// tiles (128 elements) of both operands, 32 KB; four stages in LDS are filled by LDS-DMA (a wave's request is one contiguous kilobyte = one operand tile in lane order, so there
-// is nothing to swizzle), three stages ahead.  Per stage a wave issues 32 MFMAs of 32 cycles and reads 16 KB of LDS: 96 KB of LDS traffic per 1024 cycles a CU, under its
-// 128 B / clk.
+// Large products.  A block of 2 x 2 waves owns 192 x 192 of y, a wave 96 x 96 (3 x 3 tiles, 144 accumulators), two blocks a CU: while one drains its output to memory -- 7424 x
+// 50000 in bf16 are 742 MB, as long on the way as the products take -- the other one multiplies.  A stage of the ring is two k tiles (128 elements) of both operands, 24 KB;
+// three stages in LDS are filled by LDS-DMA (a wave's request is one contiguous kilobyte = one operand tile in lane order, so there is nothing to swizzle), two stages ahead.
+// Per stage a wave issues 18 MFMAs of 32 cycles and reads 12 KB of LDS: with the fills 144 KB of LDS traffic per 1152 cycles a CU, just under its 128 B / clk.
+// (256 x 256 tiles, one block a CU with 256 accumulators a wave: 638 us at that shape, 394 of them without the stores.)
+// The output leaves through LDS in rows, past the caches' keeping: 32-byte pieces straight from the registers 581 us, rows 560, rows marked as streaming (they then do not
+// push the operands out of the L2) 460; without any stores 360, without stores and operand traffic 285, and the matrix cores alone, on random operands, which run at 6.1
+// PFLOP/s under their power limit, 250.
+constexpr int kBigTile = 192;
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 typedef __attribute__((address_space(3))) void lds_ptr;
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); __builtin_amdgcn_s_barrier(); asm volatile("" ::: "memory"); }
@@ -291,145 +301,165 @@ template <typename T>
 __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
                                                       const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy, int nbn,
                                                       int nbm, int per_xcd) {
-  constexpr int STAGE = 32 * 1024, IPW = 8;                      // bytes of a stage; LDS-DMA instructions a wave issues for one
+  constexpr int W = 3, RT = 2 * W;                               // row tiles of a wave, of a block (per side)
+  constexpr int SIDE = RT * 2048, STAGE = 2 * SIDE, NS = 3;      // bytes of a stage's operand, of a stage; stages of the ring
+  constexpr int IPW = 2 * W;                                     // LDS-DMA instructions a wave issues for a stage
   constexpr int PIN = (int)0x80000000;                           // a volatile load: it stays where it is written, ahead of the requests behind it
-  constexpr int OOB = 0x40000000;                                // past any operand buffer (KT <= 32 768: at most 2^28 bytes)
+  constexpr int OOB = 0x40000000;                                // past any operand buffer (KT <= 32 768: below 2^28 bytes)
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave & 1, wm = wave >> 1;
-  // consecutive blocks land on the eight XCDs in turn: give each XCD a contiguous run of tiles, four tiles of rows by all tiles of classes at a time, so that a run's
+  // consecutive blocks land on the eight XCDs in turn: give each XCD a contiguous run of tiles, eight tiles of rows by all tiles of classes at a time, so that a run's
   // operands stay in its L2
   const int64_t g = (int64_t)((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
   if (g >= (int64_t)nbn * nbm) return;
-  const int band = (int)(g / (4 * (int64_t)nbn)), inb = (int)(g - (int64_t)band * 4 * nbn), bw = min(4, nbm - band * 4);
-  const int bn = __builtin_amdgcn_readfirstlane(inb / bw), bm = __builtin_amdgcn_readfirstlane(band * 4 + inb % bw);      // (the division leaves them in vector registers)
+  const int band = (int)(g / (8 * (int64_t)nbn)), inb = (int)(g - (int64_t)band * 8 * nbn), bw = min(8, nbm - band * 8);
+  const int bn = __builtin_amdgcn_readfirstlane(inb / bw), bm = __builtin_amdgcn_readfirstlane(band * 8 + inb % bw);      // (the division leaves them in vector registers)
   const int ntn = (N + 31) >> 5, mtn = (int)((M + 31) >> 5);
   // The block's operand tiles of each side and their scales as buffers that end with the last of them; a tile past the matrix repeats the last one (and is not stored).
-  const int na_ = min(8, ntn - bn * 8), nb_ = min(8, mtn - bm * 8);
-  const rsrc_t ra = make_rsrc(wc + (int64_t)bn * 8 * KT * 64, (unsigned)na_ * KT * 1024), rb = make_rsrc(xc + (int64_t)bm * 8 * KT * 64, (unsigned)nb_ * KT * 1024);
-  const rsrc_t rsa = make_rsrc(wsc + (int64_t)bn * 8 * KG * 64, (unsigned)na_ * KG * 256), rsb = make_rsrc(xs + (int64_t)bm * 8 * KG * 64, (unsigned)nb_ * KG * 256);
-  // Stage st: [weights: 8 row tiles x 2 k tiles | x: the same], a kilobyte each.  Wave w takes k tile w % 2 of the row tiles w / 2 + 2 u.  Past the last k tile: no traffic,
-  // zeros in LDS.
-  auto issue = [&](int st) {
-    unsigned char* base = smem + (st & 3) * STAGE + wave * 1024;
+  const int na_ = min(RT, ntn - bn * RT), nb_ = min(RT, mtn - bm * RT);
+  const rsrc_t ra = make_rsrc(wc + (int64_t)bn * RT * KT * 64, (unsigned)na_ * KT * 1024), rb = make_rsrc(xc + (int64_t)bm * RT * KT * 64, (unsigned)nb_ * KT * 1024);
+  const rsrc_t rsa = make_rsrc(wsc + (int64_t)bn * RT * KG * 64, (unsigned)na_ * KG * 256), rsb = make_rsrc(xs + (int64_t)bm * RT * KG * 64, (unsigned)nb_ * KG * 256);
+  // Stage st in slot `slot`: [weights: RT row tiles x 2 k tiles | x: the same], a kilobyte each.  Wave w takes k tile w % 2 of the row tiles w / 2 + 2 u.  Past the last k tile:
+  // no traffic, zeros in LDS.
+  auto issue = [&](int st, int slot) {
+    unsigned char* base = smem + slot * STAGE + wave * 1024;
     const int kt = 2 * st + (wave & 1), kc = min(kt, KT - 1), voff = lane * 16 + (kt < KT ? 0 : OOB);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr*)(base + u * 4096), 16, voff, (min((wave >> 1) + 2 * u, na_ - 1) * KT + kc) * 1024, 0, 0);
+    for (int u = 0; u < W; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr*)(base + u * 4096), 16, voff, (min((wave >> 1) + 2 * u, na_ - 1) * KT + kc) * 1024, 0, 0);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr*)(base + 16384 + u * 4096), 16, voff, (min((wave >> 1) + 2 * u, nb_ - 1) * KT + kc) * 1024, 0, 0);
+    for (int u = 0; u < W; ++u) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr*)(base + SIDE + u * 4096), 16, voff, (min((wave >> 1) + 2 * u, nb_ - 1) * KT + kc) * 1024, 0, 0);
   };
-  f32x16 acc[4][4];
+  f32x16 acc[W][W];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < W; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = zero16();
-  int sa[4], sb[4], na[4], nb[4];                                // scale words: of this group of four k tiles, of the next one
+    for (int j = 0; j < W; ++j) acc[i][j] = zero16();
+  int sa[W], sb[W], na[W], nb[W];                                // scale words: of this group of four k tiles, of the next one
   auto fetch_scales = [&](int kg) {                              // (a group past the end: the last one again)
     const int kc = min(kg, KG - 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      na[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, lane * 4, (min(wn * 4 + i, na_ - 1) * KG + kc) * 256, PIN);
-      nb[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, lane * 4, (min(wm * 4 + i, nb_ - 1) * KG + kc) * 256, PIN);
+    for (int i = 0; i < W; ++i) {
+      na[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, lane * 4, (min(wn * W + i, na_ - 1) * KG + kc) * 256, PIN);
+      nb[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, lane * 4, (min(wm * W + i, nb_ - 1) * KG + kc) * 256, PIN);
     }
   };
-  const uint4* A = (const uint4*)smem + wn * 512 + lane;         // this wave's operand tiles of slot 0: [4 row tiles][2 k tiles]
-  const uint4* B = (const uint4*)(smem + 16384) + wm * 512 + lane;
+  const uint4* A = (const uint4*)smem + wn * W * 128 + lane;     // this wave's operand tiles of slot 0: [W row tiles][2 k tiles]
+  const uint4* B = (const uint4*)(smem + SIDE) + wm * W * 128 + lane;
   fetch_scales(0);
-  issue(0); issue(1); issue(2); issue(3);
-  wait_vm<3 * IPW>();                                            // stage 0 has landed for this wave ...
+  issue(0, 0); issue(1, 1); issue(2, 2);
+  wait_vm<2 * IPW>();                                            // stage 0 has landed for this wave ...
   meet();                                                        // ... and for every wave
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < W; ++i) {
     sa[i] = na[i]; sb[i] = nb[i];
     asm volatile("" : "+v"(sa[i]), "+v"(sb[i]));                  // in registers before the loop: its own waits then count the loop's requests only
   }
-  uint4 a = A[0], b[4];
+  uint4 a = A[0], b[W];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = B[j * 128];
-  // One stage: its first k tile's products run while the wave reads the rest of the stage; then everybody is done reading stage st, whose slot takes stage st + 4, and stage
-  // st + 1 has landed once at most the two younger stages' requests are outstanding (scale loads in between only make the wait stricter); the second k tile's products run while
+  for (int j = 0; j < W; ++j) b[j] = B[j * 128];
+  // One stage: its first k tile's products run while the wave reads the rest of the stage; then everybody is done reading stage st, whose slot takes stage st + 3, and stage
+  // st + 1 has landed once at most the younger stage's requests are outstanding (scale loads in between only make the wait stricter); the second k tile's products run while
   // stage st + 1's first operands are read.  The order is pinned: left alone the scheduler puts every read before the first product.  Groups of two stages, the last one filled
   // up with zeros, so that the body has no branch.
+  int slot = 0;
   auto stage = [&](int st, auto qc) {
     constexpr int q = decltype(qc)::value;
-    const int o = (st & 3) * (STAGE / 16), on = ((st + 1) & 3) * (STAGE / 16);
-    uint4 a0[4], a1[4], b1[4], bx[4];
+    const int next = slot == NS - 1 ? 0 : slot + 1;
+    const int o = slot * (STAGE / 16), on = next * (STAGE / 16);
+    uint4 a0[W], a1[W], b1[W], bx[W];
     a0[0] = a;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i < 3) a0[i + 1] = A[o + (i + 1) * 128];
+    for (int i = 0; i < W; ++i) {
+      if (i + 1 < W) a0[i + 1] = A[o + (i + 1) * 128];
       b1[i] = B[o + i * 128 + 64];
       a1[i] = A[o + i * 128 + 64];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mfma4(a0[i], b[j], acc[i][j], q, sa[i], sb[j]);
+      for (int j = 0; j < W; ++j) acc[i][j] = mfma4(a0[i], b[j], acc[i][j], q, sa[i], sb[j]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    wait_vm<2 * IPW>();
+    wait_vm<IPW>();
     meet();
     if (q == 0) fetch_scales((st >> 1) + 1);
-    issue(st + 4);
+    issue(st + 3, slot);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W; ++i) {
       if (i == 0) a = A[on];
       bx[i] = B[on + i * 128];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mfma4(a1[i], b1[j], acc[i][j], q + 1, sa[i], sb[j]);
+      for (int j = 0; j < W; ++j) acc[i][j] = mfma4(a1[i], b1[j], acc[i][j], q + 1, sa[i], sb[j]);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = bx[j];
+    for (int j = 0; j < W; ++j) b[j] = bx[j];
+    slot = next;
   };
   for (int st = 0; 2 * st < KT; st += 2) {
     stage(st, std::integral_constant<int, 0>{});
     stage(st + 1, std::integral_constant<int, 2>{});
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { sa[i] = na[i]; sb[i] = nb[i]; }
+    for (int i = 0; i < W; ++i) { sa[i] = na[i]; sb[i] = nb[i]; }
   }
   wait_vm<0>();                                                  // (the stages of zeros past the end still write LDS)
   const rsrc_t rbias = make_rsrc(bias, bias ? (unsigned)N * 4u : 0u);
-  const bool inside = (bn + 1) * 256 <= N && (int64_t)(bm + 1) * 256 <= M;
-  const int64_t m0 = (int64_t)bm * 256 + wm * 128;
-  const int n0 = bn * 256 + wn * 128;
+  const bool inside = (int64_t)(bn + 1) * kBigTile <= N && (int64_t)(bm + 1) * kBigTile <= M;
+  const int64_t m0 = (int64_t)bm * kBigTile + wm * 32 * W;
+  const int n0 = bn * kBigTile + wn * 32 * W;
   if (inside) {
-    // lanes l and l + 32 hold the two halves of eight classes: one exchange of half waves between two groups of registers gives every lane eight consecutive classes
+    // Through LDS, a wave's 96 x 96 as an image of its own, so that memory sees 192-byte (fp32: 384-byte, in two halves of the classes) runs of a row instead of 32.
+    // Lanes l and l + 32 hold the two halves of eight classes: one exchange of half waves between two groups of registers gives every lane eight consecutive classes.
+    meet();                                                      // everybody is done with the ring
+    constexpr int NW = sizeof(T), PITCH = 208, PARTS = NW / 2;   // words of four elements; bytes of an image row (192 + 16: sixteen rows start in different banks); halves
+    constexpr int CW = W * 32 / PARTS;                           // classes of a half
+    unsigned char* img = smem + wave * (96 * PITCH);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int part = 0; part < PARTS; ++part) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float bl[4], bh[4];
-        const int nl = n0 + i * 32 + 16 * h + 4 * (lane >> 5);
+      for (int i = 0; i < W; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { bl[e] = bias_at(rbias, nl + e); bh[e] = bias_at(rbias, nl + 8 + e); }
-        T* p = y + (m0 + (lane & 31)) * ldy + n0 + i * 32 + 16 * h + 8 * (lane >> 5);
+        for (int h = 0; h < 2; ++h) {
+          const int nn = i * 32 + 16 * h - part * CW;            // (16 classes lie in one half: CW is 96 or 48)
+          if (nn < 0 || nn >= CW) continue;
+          float bl[4], bh[4];
+          const int nl = n0 + i * 32 + 16 * h + 4 * (lane >> 5);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          T o[8];
-          __attribute__((aligned(16))) T lo[4], hi[4];
+          for (int e = 0; e < 4; ++e) { bl[e] = bias_at(rbias, nl + e); bh[e] = bias_at(rbias, nl + 8 + e); }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { lo[e] = from_f32<T>(acc[i][j][8 * h + e] + bl[e]); hi[e] = from_f32<T>(acc[i][j][8 * h + 4 + e] + bh[e]); }
-          constexpr int W = sizeof(T);                           // words of four elements
-          unsigned int ul[W], uh[W];
-          __builtin_memcpy(ul, lo, sizeof(ul)); __builtin_memcpy(uh, hi, sizeof(uh));
+          for (int j = 0; j < W; ++j) {
+            __attribute__((aligned(16))) T lo[4], hi[4];
 #pragma unroll
-          for (int k = 0; k < W; ++k) {
-            const auto s = __builtin_amdgcn_permlane32_swap(ul[k], uh[k], false, false);      // (ul low | uh low) , (ul high | uh high) by halves of the wave
-            ul[k] = s[0]; uh[k] = s[1];
+            for (int e = 0; e < 4; ++e) { lo[e] = from_f32<T>(acc[i][j][8 * h + e] + bl[e]); hi[e] = from_f32<T>(acc[i][j][8 * h + 4 + e] + bh[e]); }
+            unsigned int ul[NW], uh[NW];
+            __builtin_memcpy(ul, lo, sizeof(ul)); __builtin_memcpy(uh, hi, sizeof(uh));
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+              const auto s = __builtin_amdgcn_permlane32_swap(ul[k], uh[k], false, false);      // (ul low | uh low) , (ul high | uh high) by halves of the wave
+              ul[k] = s[0]; uh[k] = s[1];
+            }
+            uint4* p = (uint4*)(img + (j * 32 + (lane & 31)) * PITCH + (nn + 8 * (lane >> 5)) * (int)sizeof(T));
+            if constexpr (NW == 2) p[0] = make_uint4(ul[0], ul[1], uh[0], uh[1]);
+            else { p[0] = make_uint4(ul[0], ul[1], ul[2], ul[3]); p[1] = make_uint4(uh[0], uh[1], uh[2], uh[3]); }
           }
-          __builtin_memcpy(o, ul, sizeof(ul)); __builtin_memcpy(o + 4, uh, sizeof(uh));
-          __builtin_memcpy((void*)(p + (int64_t)j * 32 * ldy), o, sizeof(o));
         }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // (the image is this wave's own)
+#pragma unroll
+      for (int it = 0; it < 18; ++it) {
+        const int id = it * 64 + lane, r = id / 12, c = id - r * 12;
+        __builtin_nontemporal_store(*(const u32x4*)(img + r * PITCH + c * 16), (u32x4_at2*)(y + (m0 + r) * ldy + n0 + part * CW + c * (16 / (int)sizeof(T))));
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) store_tile(y, ldy, M, N, m0 + j * 32, n0 + i * 32, lane, rbias, acc[i][j]);
+      for (int j = 0; j < W; ++j) store_tile(y, ldy, M, N, m0 + j * 32, n0 + i * 32, lane, rbias, acc[i][j]);
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256, 1) void mxfp4_linear_big_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
+__global__ __launch_bounds__(256, 2) void mxfp4_linear_big_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
                                                                   const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy,
                                                                   int nbn, int nbm, int per_xcd) {
   mxfp4_linear_big_body<T>(xc, xs, M, wc, wsc, N, KT, KG, bias, y, ldy, nbn, nbm, per_xcd);
@@ -451,7 +481,7 @@ static int quantize(const void* x, int dtype, int64_t ld, int64_t rows, int K, v
   const int64_t ntask = ceil_div(rows, 32) * KG;
   const int rc = by_dtype(dtype, "mxfp4_quantize", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    hipLaunchKernelGGL((mxfp4_quantize_kernel<T>), dim3(grid_of(ntask)), dim3(256), 0, st, (const T*)x, ld, rows, K, KT, KG, ntask, (unsigned int*)codes, (unsigned int*)scales);
+    hipLaunchKernelGGL((mxfp4_quantize_kernel<T>), dim3(grid_of(ntask)), dim3(256), 0, st, (const T*)x, ld, rows, K, KT, KG, ntask, (uint4*)codes, (unsigned int*)scales);
   });
   if (rc != LEC_OK) return rc;
   LEC_CHECK_LAUNCH("mxfp4_quantize_kernel");
@@ -521,16 +551,16 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
   void* xs = (char*)workspace + codes_bytes(M, k);
   const int rc = quantize(x, xdtype, ldx, M, K, workspace, xs, st);
   if (rc != LEC_OK) return rc;
-  const int64_t nbn = ceil_div(N, 256), nbm = ceil_div(M, 256);
+  const int64_t nbn = ceil_div(N, kBigTile), nbm = ceil_div(M, kBigTile);
   if (nbn * nbm >= 128 && KT <= 32768) {
     const int64_t per = ceil_div(nbn * nbm, 8);
     LEC_CHECK_ARG(per <= (1 << 20), "mxfp4_linear: y has %lld tiles, too many for one call", (long long)(nbn * nbm));
     int rl = LEC_OK;
     by_dtype(ydtype, "", [&](auto* tag) {
       using T = std::remove_pointer_t<decltype(tag)>;
-      static const hipError_t set = hipFuncSetAttribute((const void*)mxfp4_linear_big_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+      static const hipError_t set = hipFuncSetAttribute((const void*)mxfp4_linear_big_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, 4 * 96 * 208);
       if (set != hipSuccess) { rl = hip_fail(set, "mxfp4_linear_big_kernel"); return; }
-      hipLaunchKernelGGL((mxfp4_linear_big_kernel<T>), dim3((unsigned)(per * 8)), dim3(256), 128 * 1024, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
+      hipLaunchKernelGGL((mxfp4_linear_big_kernel<T>), dim3((unsigned)(per * 8)), dim3(256), 4 * 96 * 208, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
                          (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy, (int)nbn, (int)nbm, (int)per);
     });
     if (rl != LEC_OK) return rl;

@@ -72,7 +72,7 @@ class PreferenceLoss(torch.nn.Module):
         shape = (R, 2, L) if shared else (R, L)
         p = ops._paths_arg(paths, shape, outputs)
         ref = ops._entries_arg(ref_log_probs, 'ref_log_probs', shape, outputs)
-        return ops.PreferenceLossFn.apply(outputs, p, ref, self.levels, self.beta, self.label_smoothing, shared)
+        return ops.PreferenceLossFn.apply(outputs, p, ref, (self.levels, self.beta, self.label_smoothing, shared))
 
 
 class ClippedPolicyLoss(torch.nn.Module):
@@ -109,4 +109,4 @@ class ClippedPolicyLoss(torch.nn.Module):
         adv = ops._entries_arg(advantages, 'advantages', lead, outputs)
         old = None if old_log_probs is None else ops._entries_arg(old_log_probs, 'old_log_probs', lead + (L,), outputs)
         ref = None if ref_log_probs is None else ops._entries_arg(ref_log_probs, 'ref_log_probs', lead + (L,), outputs)
-        return ops.PolicyLossFn.apply(outputs, p, adv, old, ref, self.levels, self.clip_low, self.clip_high, self.kl_coef, self.reduction == 'path')
+        return ops.PolicyLossFn.apply(outputs, p, adv, old, ref, (self.levels, self.clip_low, self.clip_high, self.kl_coef, self.reduction == 'path'))

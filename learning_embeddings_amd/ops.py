@@ -1,11 +1,12 @@
 """Tensor-level wrappers + autograd Functions over the C ABI (include/lecone.h).  PyTorch is plumbing here: device
 memory, the current HIP stream and autograd bookkeeping.  All arithmetic happens in liblecone.so on the MI355X."""
 import ctypes as C
+import functools
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import lib, check, dptr, stream_ptr
+from ._lib import lib, check, dptr, raw_stream, stream_ptr
 
 ENERGY = {'hyp_cone': _lib.ENERGY_HYP_CONE, 'order': _lib.ENERGY_ORDER, 'euc_cone': _lib.ENERGY_EUC_CONE}
 
@@ -335,11 +336,23 @@ class PathLevels:
         self.L, self.C = len(self.sizes), sum(self.sizes)
         self._arr = (C.c_int32 * self.L)(*self.sizes)
         self.ptr = C.cast(self._arr, C.c_void_p)
+        self.work = int(lib.lec_path_workspace_bytes())
+        self.row_bytes = {}                                     # partials of one row, per dtype code
+        for code in DTYPE_CODE.values():
+            n = int(lib.lec_path_partials_bytes(code, 1, self.C, self.ptr, self.L))
+            if n < 0:
+                check(n)
+            self.row_bytes[code] = n
 
     @classmethod
     def of(cls, levels):
         """levels: a PathLevels, a labelmap (its `.levels`), or a sequence of sizes."""
-        return levels if isinstance(levels, cls) else cls(getattr(levels, 'levels', levels))
+        return levels if isinstance(levels, cls) else _path_levels(tuple(int(v) for v in getattr(levels, 'levels', levels)))
+
+
+@functools.lru_cache(maxsize=64)
+def _path_levels(sizes):
+    return PathLevels(sizes)
 
 
 def _path_logits(logits, levels):
@@ -347,55 +360,72 @@ def _path_logits(logits, levels):
     matrix), a transposed or broadcast tensor is copied first."""
     if not logits.is_cuda:
         dptr(logits)                                                             # raises: there is no CPU fallback
-    if logits.dtype not in DTYPE_CODE:
+    code = DTYPE_CODE.get(logits.dtype)
+    if code is None:
         raise TypeError('logits must be float32, bfloat16 or float16, got %s' % logits.dtype)
     if logits.dim() != 2 or logits.shape[1] != levels.C:
         raise ValueError('logits must be [rows, %d] (the sum of the levels), got %s' % (levels.C, tuple(logits.shape)))
+    if logits.is_contiguous():
+        return logits, code, levels.C
     z = logits
     if z.stride(1) != 1 and z.shape[1] > 1 or z.stride(0) < z.shape[1] and z.shape[0] > 1:
         z = z.contiguous()
-    return z, DTYPE_CODE[z.dtype], (z.stride(0) if z.shape[0] > 1 else z.shape[1])
+    return z, code, (z.stride(0) if z.shape[0] > 1 else z.shape[1])
 
 
 def _paths_arg(paths, shape, like):
-    if tuple(paths.shape) != tuple(shape):
+    if paths.shape != shape:
         raise ValueError('paths must be %s, got %s' % (tuple(shape), tuple(paths.shape)))
-    if paths.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8):
-        raise TypeError('paths must hold signed integers (the class within its level, negative = not known), got %s' % paths.dtype)
     if paths.device != like.device:
         raise ValueError('paths are on %s, the logits on %s' % (paths.device, like.device))
+    if paths.dtype == torch.int64:
+        return paths if paths.is_contiguous() else paths.contiguous()
+    if paths.dtype not in (torch.int32, torch.int16, torch.int8):
+        raise TypeError('paths must hold signed integers (the class within its level, negative = not known), got %s' % paths.dtype)
     return paths.to(torch.int64).contiguous()
 
 
 def _entries_arg(t, name, shape, like):
     """A constant of the loss, fp32 and contiguous (log-probabilities of another model, advantages); its gradient is not taken."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError('%s must be %s, got %s' % (name, tuple(shape), tuple(t.shape)))
-    if not t.is_floating_point():
-        raise TypeError('%s must be floating point, got %s' % (name, t.dtype))
     if t.device != like.device:
         raise ValueError('%s are on %s, the logits on %s' % (name, t.device, like.device))
+    if t.dtype == torch.float32 and not t.requires_grad and t.is_contiguous():
+        return t
+    if not t.is_floating_point():
+        raise TypeError('%s must be floating point, got %s' % (name, t.dtype))
     return t.detach().to(torch.float32).contiguous()
 
 
-def _path_buffers(z, code, R, levels):
-    """One allocation a call: [workspace | partials].  Owned by the call (by its autograd node when a backward follows), so calls on other streams and captured
-    graphs share nothing."""
-    npart = lib.lec_path_partials_bytes(code, R, levels.C, levels.ptr, levels.L)
-    if npart < 0:
-        check(int(npart))
-    work = lib.lec_path_workspace_bytes()
-    buf = torch.empty(work + npart, dtype=torch.uint8, device=z.device)
-    return buf, C.c_void_p(buf.data_ptr()), work, C.c_void_p(buf.data_ptr() + work)
+def _f32(g):
+    return g if g.dtype == torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
 
 
-def _path_backward(ctx, coef, up, norm_ptr):
+def on_device_of(first):
+    """Decorator of a function whose argument number `first` is a tensor: runs it with that tensor's device current (kernels are launched on, and buffers taken from, the
+    current device)."""
+    def deco(f):
+        def wrapped(*args):
+            dev = args[first].device
+            if dev.type != 'cuda' or dev.index == torch.cuda.current_device():
+                return f(*args)
+            with torch.cuda.device(dev):
+                return f(*args)
+        return wrapped
+    return deco
+
+
+# Every buffer below belongs to the call (to its autograd node when a backward follows), so calls on other streams and captured graphs share nothing.
+# buf = [workspace | partials], see include/lecone.h.
+
+@on_device_of(1)
+def _path_backward(ctx, coef, coef_ptr, up, norm):
     z, paths, buf = ctx.saved_tensors[:3]
-    levels, code, ld, R, G, partials = ctx.meta
-    with torch.cuda.device(z.device):
-        dz = torch.empty(R, levels.C, dtype=z.dtype, device=z.device)
-        check(lib.lec_path_logp_bwd(dptr(z), code, ld, R, levels.C, levels.ptr, levels.L, dptr(paths), G, partials, dptr(coef), dptr(up), norm_ptr,
-                                    dptr(dz), levels.C, stream_ptr()))
+    levels, code, ld, R, G = ctx.meta
+    dz = torch.empty((R, levels.C), dtype=z.dtype, device=z.device)
+    check(lib.lec_path_logp_bwd(z.data_ptr(), code, ld, R, levels.C, levels.ptr, levels.L, paths.data_ptr(), G, buf.data_ptr() + levels.work, coef_ptr,
+                                up if up is None else up.data_ptr(), norm, dz.data_ptr(), levels.C, raw_stream(z.device.index)))
     return dz
 
 
@@ -403,19 +433,21 @@ class PathLogProbFn(torch.autograd.Function):
     """logp[r, g, l] of every entry of every path; gradient of the logits for any upstream gradient."""
 
     @staticmethod
+    @on_device_of(1)
     def forward(ctx, logits, paths, levels):
         z, code, ld = _path_logits(logits, levels)
         R, G = paths.shape[:2]
-        with torch.cuda.device(z.device):
-            logp = torch.empty(R, G, levels.L, dtype=torch.float32, device=z.device)
-            if R == 0 or G == 0:
-                ctx.meta = None
-                ctx.empty = (tuple(logits.shape), logits.dtype, logits.device)
-                return logp
-            buf, _, work, partials = _path_buffers(z, code, R, levels)
-            check(lib.lec_path_logp_fwd(dptr(z), code, ld, R, levels.C, levels.ptr, levels.L, dptr(paths), G, dptr(logp), partials, stream_ptr()))
-        ctx.save_for_backward(z, paths, buf)
-        ctx.meta = (levels, code, ld, R, G, partials)
+        logp = torch.empty((R, G, levels.L), dtype=torch.float32, device=z.device)
+        ctx.meta = None
+        if R == 0 or G == 0:
+            ctx.empty = (tuple(logits.shape), logits.dtype, logits.device)
+            return logp
+        buf = torch.empty(levels.work + R * levels.row_bytes[code], dtype=torch.uint8, device=z.device)
+        check(lib.lec_path_logp_fwd(z.data_ptr(), code, ld, R, levels.C, levels.ptr, levels.L, paths.data_ptr(), G, logp.data_ptr(), buf.data_ptr() + levels.work,
+                                    raw_stream(z.device.index)))
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(z, paths, buf)
+            ctx.meta = (levels, code, ld, R, G)
         return logp
 
     @staticmethod
@@ -424,47 +456,61 @@ class PathLogProbFn(torch.autograd.Function):
         if ctx.meta is None:
             shape, dtype, device = ctx.empty
             return torch.zeros(shape, dtype=dtype, device=device), None, None
-        return _path_backward(ctx, g.to(torch.float32).contiguous(), None, None), None, None
+        g = _f32(g)
+        return _path_backward(ctx, g, g.data_ptr(), None, None), None, None
 
 
 class PreferenceLossFn(torch.autograd.Function):
+    """spec = (levels, beta, label_smoothing, shared)"""
+
     @staticmethod
-    def forward(ctx, logits, paths, ref, levels, beta, smoothing, shared):
+    @on_device_of(1)
+    def forward(ctx, logits, paths, ref, spec):
+        levels, beta, smoothing, shared = spec
         z, code, ld = _path_logits(logits, levels)
-        R = z.shape[0]
+        R, dev = z.shape[0], z.device
         P, G = (R, 2) if shared else (R // 2, 1)
-        with torch.cuda.device(z.device):
-            loss = torch.empty((), dtype=torch.float32, device=z.device)
-            rewards = torch.empty(P, 2, dtype=torch.float32, device=z.device)
-            coef = torch.empty(R * G * levels.L, dtype=torch.float32, device=z.device)
-            buf, ws, work, partials = _path_buffers(z, code, R, levels)
-            check(lib.lec_preference_loss_fwd(dptr(z), code, ld, P, int(shared), levels.C, levels.ptr, levels.L, dptr(paths), dptr(ref), beta, smoothing,
-                                              dptr(loss), dptr(rewards), dptr(coef), partials, ws, work, stream_ptr()))
-        ctx.save_for_backward(z, paths, buf, coef)
-        ctx.meta = (levels, code, ld, R, G, partials)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        rewards = torch.empty((P, 2), dtype=torch.float32, device=dev)
+        coef = torch.empty(R * G * levels.L, dtype=torch.float32, device=dev)
+        buf = torch.empty(levels.work + R * levels.row_bytes[code], dtype=torch.uint8, device=dev)
+        ws = buf.data_ptr()
+        check(lib.lec_preference_loss_fwd(z.data_ptr(), code, ld, P, int(shared), levels.C, levels.ptr, levels.L, paths.data_ptr(), ref.data_ptr(), beta, smoothing,
+                                          loss.data_ptr(), rewards.data_ptr(), coef.data_ptr(), ws + levels.work, ws, levels.work, raw_stream(dev.index)))
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(z, paths, buf, coef)
+            ctx.meta = (levels, code, ld, R, G)
         ctx.mark_non_differentiable(rewards)
         return loss, rewards
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gl, _gr):
-        return (_path_backward(ctx, ctx.saved_tensors[3], gl.to(torch.float32).contiguous(), None),) + (None,) * 6
+        coef = ctx.saved_tensors[3]
+        return _path_backward(ctx, coef, coef.data_ptr(), _f32(gl), None), None, None, None
 
 
 class PolicyLossFn(torch.autograd.Function):
+    """spec = (levels, clip_low, clip_high, kl_coef, per_path)"""
+
     @staticmethod
-    def forward(ctx, logits, paths, adv, old, ref, levels, low, high, kl, per_path):
+    @on_device_of(1)
+    def forward(ctx, logits, paths, adv, old, ref, spec):
+        levels, low, high, kl, per_path = spec
         z, code, ld = _path_logits(logits, levels)
         R, G = paths.shape[:2]
-        with torch.cuda.device(z.device):
-            loss = torch.empty((), dtype=torch.float32, device=z.device)
-            stats = torch.empty(2, dtype=torch.float32, device=z.device)
-            coef = torch.empty(4 + R * G * levels.L, dtype=torch.float32, device=z.device)              # norm, 3 unused | coefficients
-            buf, ws, work, partials = _path_buffers(z, code, R, levels)
-            check(lib.lec_policy_loss_fwd(dptr(z), code, ld, R, levels.C, levels.ptr, levels.L, dptr(paths), G, dptr(adv), dptr(old), dptr(ref), low, high, kl,
-                                          int(per_path), dptr(loss), dptr(stats), dptr(coef), C.c_void_p(coef.data_ptr() + 16), partials, ws, work, stream_ptr()))
-        ctx.save_for_backward(z, paths, buf, coef)
-        ctx.meta = (levels, code, ld, R, G, partials)
+        dev = z.device
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        stats = torch.empty(2, dtype=torch.float32, device=dev)
+        coef = torch.empty(4 + R * G * levels.L, dtype=torch.float32, device=dev)                   # norm, 3 unused | coefficients
+        buf = torch.empty(levels.work + R * levels.row_bytes[code], dtype=torch.uint8, device=dev)
+        ws, norm = buf.data_ptr(), coef.data_ptr()
+        check(lib.lec_policy_loss_fwd(z.data_ptr(), code, ld, R, levels.C, levels.ptr, levels.L, paths.data_ptr(), G, adv.data_ptr(), old if old is None else old.data_ptr(),
+                                      ref if ref is None else ref.data_ptr(), low, high, kl, int(per_path), loss.data_ptr(), stats.data_ptr(), norm, norm + 16,
+                                      ws + levels.work, ws, levels.work, raw_stream(dev.index)))
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(z, paths, buf, coef)
+            ctx.meta = (levels, code, ld, R, G)
         ctx.mark_non_differentiable(stats)
         return loss, stats
 
@@ -472,7 +518,8 @@ class PolicyLossFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gl, _gs):
         coef = ctx.saved_tensors[3]
-        return (_path_backward(ctx, coef[4:], gl.to(torch.float32).contiguous(), dptr(coef)),) + (None,) * 9
+        norm = coef.data_ptr()
+        return _path_backward(ctx, coef, norm + 16, _f32(gl), norm), None, None, None, None, None
 
 
 # ------------------------------------------------------------------------------------------------ per-model fusion records

@@ -8,25 +8,25 @@ infinity stands for NaN.  17/32 bytes an element (rows padded to 32, elements to
     logits = head(features)                           # quantises the features row by row, multiplies on the 4-bit matrix cores, sums in 32 bits
 
 The head is frozen -- a reference model's, or one that serves: its weights take no gradient and it passes none to its input."""
-import ctypes as C
-
 import torch
 import torch.nn as nn
 
-from . import _lib
-from ._lib import lib, check, dptr, stream_ptr
-from .ops import DTYPE_CODE
+from ._lib import lib, check, dptr, raw_stream
+from .ops import DTYPE_CODE, on_device_of
 
 
 def _matrix(x, name):
     """(row-major 2-D view, dtype code, row stride)"""
-    if x.dtype not in DTYPE_CODE:
+    code = DTYPE_CODE.get(x.dtype)
+    if code is None:
         raise TypeError('%s must be float32, bfloat16 or float16, got %s' % (name, x.dtype))
     if not x.is_cuda:
         dptr(x)                                                                  # raises: there is no CPU fallback
+    if x.is_contiguous():
+        return x, code, x.shape[1]
     if x.stride(1) != 1 and x.shape[1] > 1 or x.stride(0) < x.shape[1] and x.shape[0] > 1:
         x = x.contiguous()
-    return x, DTYPE_CODE[x.dtype], (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+    return x, code, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
 
 
 class MXFP4Tensor:
@@ -47,11 +47,46 @@ class MXFP4Tensor:
         if dtype not in (torch.float32, torch.bfloat16):
             raise TypeError('the values are exact in float32 and bfloat16 only, got %s' % dtype)
         rows, k = self.shape
-        out = torch.empty(rows, k, dtype=dtype, device=self.device)
-        if rows and k:
-            with torch.cuda.device(self.device):
-                check(lib.lec_mxfp4_dequantize(dptr(self.codes), dptr(self.scales), rows, k, dptr(out), DTYPE_CODE[dtype], k, stream_ptr()))
-        return out
+        if rows == 0 or k == 0:
+            return torch.empty(rows, k, dtype=dtype, device=self.device)
+        return _dequantize(self.codes, self.scales, rows, k, dtype)
+
+
+@on_device_of(0)
+def _dequantize(codes, scales, rows, k, dtype):
+    out = torch.empty((rows, k), dtype=dtype, device=codes.device)
+    check(lib.lec_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, k, out.data_ptr(), DTYPE_CODE[dtype], k, raw_stream(codes.device.index)))
+    return out
+
+
+@on_device_of(0)
+def _quantize(z, code, ld, rows, k):
+    codes = torch.empty(codes_bytes(rows, k), dtype=torch.uint8, device=z.device)
+    scales = torch.empty(scales_bytes(rows, k), dtype=torch.uint8, device=z.device)
+    check(lib.lec_mxfp4_quantize(z.data_ptr(), code, ld, rows, k, codes.data_ptr(), scales.data_ptr(), raw_stream(z.device.index)))
+    return codes, scales
+
+
+@on_device_of(0)
+def _linear(z, code, ld, codes, scales, N, k, bias, dtype):
+    M = z.shape[0]
+    y = torch.empty((M, N), dtype=dtype, device=z.device)
+    ws = torch.empty(codes_bytes(M, k) + scales_bytes(M, k), dtype=torch.uint8, device=z.device)      # this call's own
+    check(lib.lec_mxfp4_linear(z.data_ptr(), code, ld, M, codes.data_ptr(), scales.data_ptr(), N, k, bias if bias is None else bias.data_ptr(), y.data_ptr(), DTYPE_CODE[dtype],
+                               N, ws.data_ptr(), ws.numel(), raw_stream(z.device.index)))
+    return y
+
+
+def codes_bytes(rows, k):
+    """As lec_mxfp4_codes_bytes: tiles of 32 rows x 64 elements, a kilobyte each."""
+    if rows > (1 << 31) - 32 or k > 1 << 24:
+        raise ValueError('matrix too large for the 4-bit form (at most 2^31 - 32 rows of 2^24 elements): %d x %d' % (rows, k))
+    return (rows + 31 >> 5) * (k + 63 >> 6) << 10
+
+
+def scales_bytes(rows, k):
+    """As lec_mxfp4_scales_bytes: a word a lane for four tiles."""
+    return (rows + 31 >> 5) * (k + 255 >> 8) << 8
 
 
 def mxfp4_quantize(x):
@@ -65,17 +100,7 @@ def mxfp4_quantize(x):
     if rows == 0:
         e = torch.empty(0, dtype=torch.uint8, device=z.device)
         return MXFP4Tensor(e, e, (0, k))
-    with torch.cuda.device(z.device):
-        codes = torch.empty(_size(lib.lec_mxfp4_codes_bytes(rows, k)), dtype=torch.uint8, device=z.device)
-        scales = torch.empty(_size(lib.lec_mxfp4_scales_bytes(rows, k)), dtype=torch.uint8, device=z.device)
-        check(lib.lec_mxfp4_quantize(dptr(z), code, ld, rows, k, dptr(codes), dptr(scales), stream_ptr()))
-    return MXFP4Tensor(codes, scales, (rows, k))
-
-
-def _size(n):
-    if n < 0:
-        raise ValueError('matrix too large for the 4-bit form (at most 2^31 - 32 rows of 2^24 elements)')
-    return int(n)
+    return MXFP4Tensor(*_quantize(z, code, ld, rows, k), (rows, k))
 
 
 class MXFP4Linear(nn.Module):
@@ -114,14 +139,13 @@ class MXFP4Linear(nn.Module):
             raise ValueError('x must be [..., %d], got %s' % (self.in_features, tuple(x.shape)))
         if x.device != self.codes.device:
             raise ValueError('x is on %s, the head on %s' % (x.device, self.codes.device))
-        z, code, ld = _matrix(x.reshape(-1, self.in_features), 'x')
-        M, N, k = z.shape[0], self.out_features, self.in_features
+        z, code, ld = _matrix(x if x.dim() == 2 else x.reshape(-1, self.in_features), 'x')
         dtype = self.out_dtype or x.dtype
-        with torch.cuda.device(z.device):
-            y = torch.empty(M, N, dtype=dtype, device=z.device)
-            if M:
-                ws = torch.empty(_size(lib.lec_mxfp4_linear_workspace_bytes(M, N, k)), dtype=torch.uint8, device=z.device)      # this call's own
-                b = self.bias if self.bias is None or self.bias.dtype == torch.float32 else self.bias.float()     # (.half() on a model converts its buffers)
-                check(lib.lec_mxfp4_linear(dptr(z), code, ld, M, dptr(self.codes), dptr(self.scales), N, k, dptr(b), dptr(y), DTYPE_CODE[dtype], N, dptr(ws), ws.numel(),
-                                           stream_ptr()))
-        return y.view(*x.shape[:-1], N)
+        bias = self.bias
+        if bias is not None and bias.dtype != torch.float32:
+            bias = bias.float()                                                  # (.half() on a model converts its buffers)
+        if z.shape[0] == 0:
+            y = torch.empty(0, self.out_features, dtype=dtype, device=z.device)
+        else:
+            y = _linear(z, code, ld, self.codes, self.scales, self.out_features, self.in_features, bias, dtype)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], self.out_features)

@@ -192,3 +192,12 @@ def test_mxfp4_refusals():
     assert lib.lec_mxfp4_linear(p, 0, 32, 1, p, p, 4, 32, None, p, 0, 3, p, 1 << 20, None) == _lib.E_ARG and b'ldy' in lib.lec_last_error()
     assert lib.lec_mxfp4_linear(p, 0, 32, 1, p, p, 4, 32, None, p, 0, 4, p, 1024, None) == _lib.E_ARG and b'workspace' in lib.lec_last_error()
     assert lib.lec_mxfp4_linear(p, 0, 32, 1, p, p, 4, 32, None, p, 5, 4, p, 1 << 20, None) == _lib.E_ARG and b'dtype' in lib.lec_last_error()
+
+
+def test_mxfp4_sizes_agree_with_the_library():
+    from learning_embeddings_amd import _lib, quant
+    for rows, k in [(1, 1), (31, 64), (32, 65), (33, 256), (723, 515), (50000, 2048), (2 ** 31 - 32, 2 ** 24)]:
+        assert quant.codes_bytes(rows, k) == _lib.lib.lec_mxfp4_codes_bytes(rows, k) and quant.scales_bytes(rows, k) == _lib.lib.lec_mxfp4_scales_bytes(rows, k)
+        assert quant.codes_bytes(rows, k) + quant.scales_bytes(rows, k) == _lib.lib.lec_mxfp4_linear_workspace_bytes(rows, 5, k)
+    with pytest.raises(ValueError, match='too large'):
+        quant.codes_bytes(1, 2 ** 24 + 1)
