@@ -13,6 +13,7 @@
 // goes to `partials`, and whoever needs a level's lse merges its few runs again in the same order (the saved state of the backward pass IS `partials`).
 // Vectors start at the level's first class, which no alignment is promised for: the loads are 16 bytes wide at element alignment.
 #include "lec_common.h"
+#include "conv_geo.h"
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
 
@@ -26,20 +27,30 @@ struct PathTable {
   int start[kMaxLevels + 1];     // first class of a level
   int first[kMaxLevels + 1];     // first run of a level
   int vpr[kMaxLevels];           // 16-byte vectors of a run
+  FastDiv byS, byG;              // task / S, path / G where the tasks, the paths fit 31 bits
 };
+__device__ __forceinline__ int64_t row_of(const PathTable& t, int64_t task, int64_t ntask) { return ntask <= INT32_MAX ? (int64_t)fdiv((int)task, t.byS) : task / t.S; }
 
 template <typename T> struct Elt;
 template <> struct Elt<float> {
   static constexpr int V = 4, NL = 9;
   static __device__ __forceinline__ float get(const uint4& w, int e) { return __uint_as_float(e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w); }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  static __device__ __forceinline__ void put(uint4& w, int e, const float* p) { (e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w) = __float_as_uint(*p); }
   static __device__ __forceinline__ float load(const float* p) { return *p; }
   static __device__ __forceinline__ uint4 pack(const float (&f)[4]) { return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])); }
   static __device__ __forceinline__ float cvt(float f) { return f; }
 };
+__device__ __forceinline__ void put_half(uint4& w, int e, unsigned short h) {
+  unsigned int& u = (e >> 1) == 0 ? w.x : (e >> 1) == 1 ? w.y : (e >> 1) == 2 ? w.z : w.w;
+  u = (e & 1) ? (u & 0xffffu) | ((unsigned int)h << 16) : (u & 0xffff0000u) | h;
+}
 __device__ __forceinline__ unsigned int word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 template <> struct Elt<__hip_bfloat16> {
   static constexpr int V = 8, NL = 5;
   static __device__ __forceinline__ float get(const uint4& w, int e) { const unsigned int u = word_of(w, e >> 1); return __uint_as_float((e & 1) ? (u & 0xffff0000u) : (u << 16)); }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  static __device__ __forceinline__ void put(uint4& w, int e, const __hip_bfloat16* p) { put_half(w, e, *(const unsigned short*)p); }
   static __device__ __forceinline__ float load(const __hip_bfloat16* p) { return __uint_as_float((unsigned int)*(const unsigned short*)p << 16); }
   static __device__ __forceinline__ __hip_bfloat16 cvt(float f) { return __float2bfloat16(f); }        // nearest, ties to even; NaN stays NaN
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
@@ -59,6 +70,8 @@ template <> struct Elt<_Float16> {
     const unsigned short h = (unsigned short)((e & 1) ? (u >> 16) : (u & 0xffffu));
     return (float)__builtin_bit_cast(_Float16, h);
   }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+  static __device__ __forceinline__ void put(uint4& w, int e, const _Float16* p) { put_half(w, e, __builtin_bit_cast(unsigned short, *p)); }
   static __device__ __forceinline__ float load(const _Float16* p) { return (float)*p; }
   static __device__ __forceinline__ _Float16 cvt(float f) { return (_Float16)f; }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
@@ -72,34 +85,39 @@ template <> struct Elt<_Float16> {
 
 // 16 bytes at element alignment (the compiler emits one dwordx4 access: the target's unaligned access mode)
 template <typename T> __device__ __forceinline__ uint4 load16(const T* p) { uint4 w; __builtin_memcpy(&w, (const void*)p, 16); return w; }
+#ifdef V_NT
+typedef unsigned int u32x4s __attribute__((ext_vector_type(4)));
+typedef u32x4s u32x4s_at2 __attribute__((aligned(2)));
+template <typename T> __device__ __forceinline__ void store16(T* p, const uint4& w) { __builtin_nontemporal_store(u32x4s{w.x, w.y, w.z, w.w}, (u32x4s_at2*)p); }
+#else
 template <typename T> __device__ __forceinline__ void store16(T* p, const uint4& w) { __builtin_memcpy((void*)p, &w, 16); }
+#endif
 
 __device__ __forceinline__ float fast_exp(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }      // t <= 0: absolute error of a softmax term below 2^-23
 
-// One run: elements [lo, hi) of the level, lane-strided vectors.  x[j][e] = -inf outside.
+// One run of a level of n elements at z: vectors v0 .. v0 + nv, one in 64 a lane, raw; -inf where there is none.
 template <typename T>
 struct Run {
   static constexpr int V = Elt<T>::V, NL = Elt<T>::NL;
-  float x[NL][V];
-  __device__ __forceinline__ void load(const T* z, int v0, int nv, int n, int lane) {     // vectors v0 .. v0 + nv of a level of n elements at z
-    uint4 w[NL];
+  uint4 w[NL];
+  __device__ __forceinline__ void load(const T* z, int v0, int nv, int n, int lane) {
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int k = j * 64 + lane, e0 = (v0 + k) * V;
+      w[j] = Elt<T>::none();
       if (k < nv && e0 + V <= n) w[j] = load16(z + e0);
     }
+    const int last = n / V - v0;                                 // the level's last, incomplete vector, if it has one and it is this run's
+    if (n % V && last < nv && (last & 63) == lane) {
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int k = j * 64 + lane, e0 = (v0 + k) * V;
-      const bool full = k < nv && e0 + V <= n;
+      for (int j = 0; j < NL; ++j)
+        if (j == last >> 6) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[j][e] = full ? Elt<T>::get(w[j], e) : -INFINITY;
-      if (k < nv && !full) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) if (e0 + e < n) x[j][e] = Elt<T>::load(z + e0 + e);
-      }
+          for (int e = 0; e < V - 1; ++e) if (e < n % V) Elt<T>::put(w[j], e, z + (v0 + last) * V + e);
+        }
     }
   }
+  __device__ __forceinline__ float get(int j, int e) const { return Elt<T>::get(w[j], e); }
 };
 
 __device__ __forceinline__ int level_of(const PathTable& t, int slot) {
@@ -109,12 +127,12 @@ __device__ __forceinline__ int level_of(const PathTable& t, int slot) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z, int64_t ld, int64_t R, PathTable t, float2* __restrict__ partials, unsigned int* counter) {
+__global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z, int64_t ld, int64_t R, PathTable t, float2* __restrict__ partials, unsigned int* counters) {
   const int lane = threadIdx.x & 63;
-  if (counter && blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;              // armed for the loss kernel behind this launch
+  if (counters && blockIdx.x == 0 && threadIdx.x <= 32) counters[threadIdx.x * 32] = 0;      // armed for the loss kernel behind this launch (grid_sum)
   const int64_t ntask = R * t.S, nwave = (int64_t)gridDim.x * 4;
   for (int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); task < ntask; task += nwave) {
-    const int64_t r = task / t.S;
+    const int64_t r = row_of(t, task, ntask);
     const int slot = (int)(task - r * t.S), l = level_of(t, slot), n = t.start[l + 1] - t.start[l];
     constexpr int V = Elt<T>::V, NL = Elt<T>::NL;
     const int v0 = (slot - t.first[l]) * t.vpr[l], nv = min(t.vpr[l], (n + V - 1) / V - v0);
@@ -124,7 +142,7 @@ __global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z
 #pragma unroll
     for (int j = 0; j < NL; ++j)
 #pragma unroll
-      for (int e = 0; e < V; ++e) m = fmaxf(m, run.x[j][e]);
+      for (int e = 0; e < V; ++e) m = fmaxf(m, run.get(j, e));
     m = group_max<64>(m);
     const float mm = m == -INFINITY ? 0.0f : m;                                  // nothing finite: the terms are exp(-inf) = 0 (NaN stays NaN)
     float s = 0.0f;
@@ -132,31 +150,51 @@ __global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z
     for (int j = 0; j < NL; ++j)
       if (j * 64 < nv) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += fast_exp(run.x[j][e] - mm);
+        for (int e = 0; e < V; ++e) s += fast_exp(run.get(j, e) - mm);
       }
     s = group_sum<64>(s);
     if (lane == 0) partials[task] = make_float2(m, s);
   }
 }
 
-// (max, sum) of a whole level from its runs, in the order of the runs
+// (max, sum) of a whole level from its n runs, eight at a time (their loads in flight together), in the order of the runs
 __device__ __forceinline__ float2 merge_runs(const float2* __restrict__ p, int n) {
-  float m = -INFINITY;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, p[i].x);
-  float s = 0.0f;
-  for (int i = 0; i < n; ++i) {
-    const float2 q = p[i];
-    s += q.x == m ? q.y : q.y * fast_exp(q.x - m);                               // (q.x = -inf beside a finite m: 0 * exp(-inf) = 0)
+  float m = -INFINITY, s = 0.0f;
+  for (int i = 0; i < n; i += 8) {
+    float2 q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = p[min(i + j, n - 1)];
+    float mq = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mq = fmaxf(mq, q[j].x);
+    s = m == mq ? s : s * fast_exp(m - mq);                                      // (m = -inf beside a finite mq: 0)
+    m = mq;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (i + j < n) s += q[j].x == m ? q[j].y : q[j].y * fast_exp(q[j].x - m);
   }
   return make_float2(m, s);
 }
+// The same by a wave: lane i takes run i (a level of more than 64 runs: the lane merges every 64th first)
+__device__ __forceinline__ float2 merge_runs_wave(const float2* __restrict__ p, int n, int lane) {
+  float m = -INFINITY, s = 0.0f;
+  for (int i = lane; i < n; i += 64) {
+    const float2 q = p[i];
+    const float mq = fmaxf(m, q.x);
+    s = (m == mq ? s : s * fast_exp(m - mq)) + (q.x == mq ? q.y : q.y * fast_exp(q.x - mq));
+    m = mq;
+  }
+  const float mw = group_max<64>(m);
+  return make_float2(mw, group_sum<64>(m == mw ? s : s * fast_exp(m - mw)));
+}
 
-// log-probability of class y of level l of row r in 64 bits: (z - m) - log s
+// log-probability of class y of level l of row r in 64 bits: (z - m) - log s; NaN where the level has no such class
+template <typename T>
+__device__ __forceinline__ float named_logit(const T* __restrict__ z, int64_t ld, int64_t r, const PathTable& t, int l, int64_t y) {
+  return y < t.start[l + 1] - t.start[l] ? Elt<T>::load(z + r * ld + t.start[l] + y) : __builtin_nanf("");
+}
 template <typename T>
 __device__ __forceinline__ double entry_logp(const T* __restrict__ z, int64_t ld, int64_t r, const PathTable& t, int l, int64_t y, const float2* __restrict__ partials) {
-  const int n = t.start[l + 1] - t.start[l];
-  if (y >= n) return __builtin_nan("");
-  const float zy = Elt<T>::load(z + r * ld + t.start[l] + y);
+  const float zy = named_logit(z, ld, r, t, l, y);
   const float2 ms = merge_runs(partials + r * t.S + t.first[l], t.first[l + 1] - t.first[l]);
   return ((double)zy - (double)ms.x) - log((double)ms.y);
 }
@@ -171,10 +209,14 @@ __global__ __launch_bounds__(256) void path_logp_kernel(const T* __restrict__ z,
   }
 }
 
-// Sum of N doubles over the grid in a fixed order; true in thread 0 of the last block, `total` valid there.  Same hand-off as block_publish_and_finalize
-// (lec_common.h); `counter` was zeroed by the launch before.  All threads of the block call it (256 threads).
+// Sum of N doubles over the grid in a fixed order; true in one thread of the last block to arrive, `total` valid there.  `counters` were zeroed by the launch before.  All
+// threads of the block call it (256 threads).  A block draws a ticket from one of 32 counters, a cache line each, and the last of each counter one from a 33rd: tickets of one
+// word are drawn one after the other, 2 048 of them in 20 us (up to 64 blocks share one).  The blocks' sums are handed over by agent-scope accesses alone, which act at the coherence point past the XCDs' L2s: a sum is
+// there (vmcnt 0) before its block's ticket is drawn, and the last block asks for the sums after its own ticket has come back.  A release fence in every block would say the
+// same and write the whole L2 back each time: 2 048 blocks spent 45 of 57 us on it.
+constexpr unsigned int kTickets = 32;
 template <int N>
-__device__ __forceinline__ bool grid_sum(double (&v)[N] /* one value a thread */, double* __restrict__ block_sums, unsigned int* counter, double (&total)[N]) {
+__device__ __forceinline__ bool grid_sum(double (&v)[N] /* one value a thread */, double* __restrict__ block_sums, unsigned int* counters, double (&total)[N]) {
   __shared__ double s_w[4][N];
   __shared__ int s_last;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -186,50 +228,64 @@ __device__ __forceinline__ bool grid_sum(double (&v)[N] /* one value a thread */
   __syncthreads();
   if (threadIdx.x == 0) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) block_sums[(int64_t)blockIdx.x * N + k] = s_w[0][k] + s_w[1][k] + s_w[2][k] + s_w[3][k];
+    for (int k = 0; k < N; ++k)
+      __hip_atomic_store(&block_sums[(int64_t)blockIdx.x * N + k], s_w[0][k] + s_w[1][k] + s_w[2][k] + s_w[3][k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const unsigned int prev = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = prev == gridDim.x - 1;
-    if (s_last) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
+    const unsigned int groups = gridDim.x <= 64 ? 1 : kTickets, g = blockIdx.x % groups, of_g = (gridDim.x - g + groups - 1) / groups;
+    int last = __hip_atomic_fetch_add(counters + g * 32, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of_g - 1;
+    if (last && groups > 1) last = __hip_atomic_fetch_add(counters + kTickets * 32, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+    s_last = last;
   }
   __syncthreads();
-  if (!s_last || w != 0) return false;
+  if (!s_last) return false;
+  double part[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) total[k] = 0.0;
-  for (unsigned int i = lane; i < gridDim.x; i += 64)
+  for (int k = 0; k < N; ++k) part[k] = 0.0;
+  for (unsigned int i0 = 0; i0 < gridDim.x; i0 += 1024) {                        // four blocks' sums a thread, in flight together
+    double q[4][N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) total[k] += block_sums[(int64_t)i * N + k];
+    for (int j = 0; j < 4; ++j) {
+      const unsigned int i = i0 + 256 * j + threadIdx.x;
 #pragma unroll
-  for (int k = 0; k < N; ++k)
-    for (int m = 32; m >= 1; m >>= 1) total[k] += __shfl_xor(total[k], m, 64);
-  return lane == 0;
+      for (int k = 0; k < N; ++k) q[j][k] = i < gridDim.x ? __hip_atomic_load(&block_sums[(int64_t)i * N + k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < N; ++k) part[k] += q[j][k];
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    for (int m = 32; m >= 1; m >>= 1) part[k] += __shfl_xor(part[k], m, 64);
+    if (lane == 0) s_w[w][k] = part[k];                          // (s_w was read before the barrier above)
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) total[k] = s_w[0][k] + s_w[1][k] + s_w[2][k] + s_w[3][k];
+  return threadIdx.x == 0;
 }
 
 // Preference loss.  Pair p: reward of a side = beta * sum_l (logp - ref), d = chosen - rejected,
 //   loss = mean_p (1 - eps) softplus(-d) + eps softplus(d) ;  d loss / d d = (eps sigma(d) - (1 - eps) sigma(-d)) / P .
-// 16 lanes a side (one a level), 32 a pair.  shared: both paths score row p; otherwise rows p and P + p.
+// A side is LW = the power of two >= L lanes (one a level), a pair 2 LW.  shared: both paths score row p; otherwise rows p and P + p.
 template <typename T>
-__global__ __launch_bounds__(256) void preference_kernel(const T* __restrict__ z, int64_t ld, int64_t P, int shared, PathTable t, const int64_t* __restrict__ paths,
+__global__ __launch_bounds__(256) void preference_kernel(const T* __restrict__ z, int64_t ld, int64_t P, int shared, int LW, PathTable t, const int64_t* __restrict__ paths,
                                                          const float* __restrict__ ref, float beta, float eps, const float2* __restrict__ partials, float* __restrict__ coef,
-                                                         float* __restrict__ rewards, float* __restrict__ loss, double* __restrict__ block_sums, unsigned int* counter) {
-  const int l = threadIdx.x & 15, side = (threadIdx.x >> 4) & 1;
+                                                         float* __restrict__ rewards, float* __restrict__ loss, double* __restrict__ block_sums, unsigned int* counters) {
+  const int sh = 31 - __builtin_clz(LW), l = threadIdx.x & (LW - 1), side = (threadIdx.x >> sh) & 1, per_block = 128 >> sh;
   double acc[1] = {0.0};
   // every lane of a wave takes part in the shuffles: the loop bound is the block's, a lane past the last pair works on nothing
-  for (int64_t p0 = (int64_t)blockIdx.x * 8; p0 < P; p0 += (int64_t)gridDim.x * 8) {
-    const int64_t p = p0 + (threadIdx.x >> 5);
+  for (int64_t p0 = (int64_t)blockIdx.x * per_block; p0 < P; p0 += (int64_t)gridDim.x * per_block) {
+    const int64_t p = p0 + (threadIdx.x >> (sh + 1));
     const bool in = p < P && l < t.L;
     const int64_t row = shared ? p : side * P + p, entry = ((shared ? p * 2 + side : row)) * t.L + l;
     const int64_t y = in ? paths[entry] : -1;
+    const double rf = in ? (double)ref[entry] : 0.0;
     double r = 0.0;
-    if (y >= 0) r = entry_logp(z, ld, row, t, l, y, partials) - (double)ref[entry];
-    for (int m = 8; m >= 1; m >>= 1) r += __shfl_xor(r, m, 16);
+    if (y >= 0) r = entry_logp(z, ld, row, t, l, y, partials) - rf;
+    for (int m = LW >> 1; m >= 1; m >>= 1) r += __shfl_xor(r, m, LW);
     r *= (double)beta;
-    const double other = __shfl_xor(r, 16, 32), d = side ? other - r : r - other;
+    const double other = __shfl_xor(r, LW, 2 * LW), d = side ? other - r : r - other;
     const double e = exp(-fabs(d)), lp = log1p(e);                               // softplus(-d) = max(-d, 0) + log1p(exp(-|d|))
     const double sp = 1.0 / (1.0 + e), sm = e / (1.0 + e);                       // sigma(|d|), sigma(-|d|)
     const double sig = d >= 0.0 ? sp : (d < 0.0 ? sm : d), sigm = d >= 0.0 ? sm : (d < 0.0 ? sp : d);      // (NaN stays NaN)
@@ -242,37 +298,71 @@ __global__ __launch_bounds__(256) void preference_kernel(const T* __restrict__ z
     }
   }
   double total[1];
-  if (grid_sum<1>(acc, block_sums, counter, total)) loss[0] = (float)(total[0] / (double)P);
+  if (grid_sum<1>(acc, block_sums, counters, total)) loss[0] = (float)(total[0] / (double)P);
 }
 
 // Clipped policy loss.  Entry (r, g, l) counted: rho = exp(logp - old), A = advantage[r, g],
 //   t = -min(rho A, clip(rho, 1 - lo, 1 + hi) A) + kl (exp(q) - q - 1),  q = ref - logp ;  dt/dlogp = -rho A [inside or on the bound] - kl expm1(q)
 // loss = sum w t.  mean over counted entries: w = 1 / N, N known only at the end of this launch -- c is left without it and `norm` = 1 / max(N, 1) multiplies it in
 // the backward pass; mean over paths: w = 1 / (entries of the path) / (R G), norm = 1.  stats = {sum w k3, sum w [clipped]}.
-// A path is LW = the power of two >= L lanes of a wave.
+// A path is LW = the power of two >= L lanes of a wave.  The block's paths belong to a few consecutive rows: it first merges the runs of those rows' levels into LDS, as many
+// lanes to a level as there are for it (a lane that merged its own level would wait for the level of the most runs, sixteen times over for sixteen paths of a row).
 template <typename T>
 __global__ __launch_bounds__(256) void policy_kernel(const T* __restrict__ z, int64_t ld, int64_t n_paths, int LW, PathTable t, const int64_t* __restrict__ paths,
                                                      const float* __restrict__ adv, const float* __restrict__ old, const float* __restrict__ ref, float lo, float hi, float kl,
-                                                     int per_path, const float2* __restrict__ partials, float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ stats, float* __restrict__ norm,
-                                                     double* __restrict__ block_sums, unsigned int* counter) {
-  const int l = threadIdx.x & (LW - 1), per_block = 256 / LW;
-  const int sh = 31 - __builtin_clz(LW);
+                                                     int per_path, const float2* __restrict__ partials, float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ stats,
+                                                     float* __restrict__ norm, double* __restrict__ block_sums, unsigned int* counters) {
+  __shared__ double s_lse[256][2];                               // (m, log s) of the block's rows' levels: at most 256 (G = 1: one a lane; G > 1: half of that and two rows)
+  const int sh = 31 - __builtin_clz(LW), l = threadIdx.x & (LW - 1), per_block = 256 >> sh;
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
   for (int64_t q0 = (int64_t)blockIdx.x * per_block; q0 < n_paths; q0 += (int64_t)gridDim.x * per_block) {
     const int64_t q = q0 + (threadIdx.x >> sh);
     const bool in = q < n_paths && l < t.L;
-    const int64_t entry = q * t.L + l, y = in ? paths[entry] : -1, row = q / t.G;
+    const int64_t entry = q * t.L + l, y = in ? paths[entry] : -1;
+    const auto row_at = [&](int64_t path) { return n_paths <= INT32_MAX ? (int64_t)fdiv((int)path, t.byG) : path / t.G; };
+    const int64_t row = row_at(in ? q : q0), row0 = row_at(q0), row1 = row_at(min(q0 + per_block, n_paths) - 1);
     const bool on = y >= 0;
+    double A = 0.0, lo_ = 0.0, lr_ = 0.0;
+    float zy = 0.0f;
+    if (on) {                                                    // asked for before the merge below
+      A = (double)adv[q];
+      if (old) lo_ = (double)old[entry];
+      if (ref) lr_ = (double)ref[entry];
+      zy = named_logit(z, ld, row, t, l, y);
+    }
+    const int units = (int)(row1 - row0 + 1) * t.L;
+    int LP = 256;                                                // lanes to a unit
+    while (LP > 64 || LP * units > 256) LP >>= 1;
+    const int u = threadIdx.x / LP, ul = u % t.L, i0 = threadIdx.x & (LP - 1);
+    float m = -INFINITY, s = 0.0f;
+    if (u < units) {
+      const float2* pr = partials + (row0 + u / t.L) * t.S + t.first[ul];
+      const int n = t.first[ul + 1] - t.first[ul];
+      for (int i = i0; i < n; i += LP) {
+        const float2 v = pr[i];
+        const float mv = fmaxf(m, v.x);
+        s = (m == mv ? s : s * fast_exp(m - mv)) + (v.x == mv ? v.y : v.y * fast_exp(v.x - mv));
+        m = mv;
+      }
+    }
+    for (int w = LP >> 1; w >= 1; w >>= 1) {
+      const float mo = __shfl_xor(m, w, 64), so = __shfl_xor(s, w, 64), mv = fmaxf(m, mo);
+      const float own = m == mv ? s : s * fast_exp(m - mv), oth = mo == mv ? so : so * fast_exp(mo - mv);
+      s = own + oth; m = mv;                                     // (a sum of two: the same in both lanes)
+    }
+    if (u < units && i0 == 0) { s_lse[u][0] = (double)m; s_lse[u][1] = log((double)s); }
+    __syncthreads();
     const unsigned long long mask = __ballot(on) >> ((threadIdx.x & 63) & ~(LW - 1));
     const int cnt = __popcll(mask & ((1ull << LW) - 1ull));
     float c = 0.0f;
     if (on) {
-      const double lp = entry_logp(z, ld, row, t, l, y, partials), A = (double)adv[q];
-      const double rho = old ? exp(lp - (double)old[entry]) : exp(lp - lp);       // (no old log-probabilities: on-policy, the ratio is 1)
+      const int k = (int)(row - row0) * t.L + l;
+      const double lp = ((double)zy - s_lse[k][0]) - s_lse[k][1];
+      const double rho = exp(lp - (old ? lo_ : lp));                              // (no old log-probabilities: on-policy, the ratio is 1)
       const bool clipped = (A > 0.0 && rho > 1.0 + (double)hi) || (A < 0.0 && rho < 1.0 - (double)lo);
       const double gain = clipped ? (A > 0.0 ? 1.0 + (double)hi : 1.0 - (double)lo) * A : rho * A;
       double k3 = 0.0, dk = 0.0;
-      if (ref) { const double d = (double)ref[entry] - lp, em = expm1(d); k3 = em - d; dk = em; }
+      if (ref) { const double d = lr_ - lp, em = expm1(d); k3 = em - d; dk = em; }
       const double w = per_path ? 1.0 / ((double)cnt * (double)n_paths) : 1.0;
       acc[0] += w * ((kl != 0.0f ? (double)kl * k3 : 0.0) - gain);
       acc[1] += w * k3;
@@ -281,9 +371,10 @@ __global__ __launch_bounds__(256) void policy_kernel(const T* __restrict__ z, in
       c = (float)(w * ((clipped ? 0.0 : -rho * A) - (kl != 0.0f ? (double)kl * dk : 0.0)));
     }
     if (in) coef[entry] = c;
+    __syncthreads();                                             // (the next round writes s_lse)
   }
   double total[4];
-  if (grid_sum<4>(acc, block_sums, counter, total)) {
+  if (grid_sum<4>(acc, block_sums, counters, total)) {
     const double inv = per_path ? 1.0 : 1.0 / (total[3] > 1.0 ? total[3] : 1.0);
     loss[0] = (float)(total[0] * inv); stats[0] = (float)(total[1] * inv); stats[1] = (float)(total[2] * inv); norm[0] = (float)inv;
   }
@@ -302,7 +393,7 @@ __global__ __launch_bounds__(256) void path_grad_kernel(const T* __restrict__ z,
   const float scale = (up ? *up : 1.0f) * (norm ? *norm : 1.0f);
   for (int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); task < ntask; task += nwave) {
     constexpr int V = Elt<T>::V, NL = Elt<T>::NL;
-    const int64_t r = task / t.S;
+    const int64_t r = row_of(t, task, ntask);
     const int slot = (int)(task - r * t.S), l = level_of(t, slot), n = t.start[l + 1] - t.start[l];
     const int v0 = (slot - t.first[l]) * t.vpr[l], nv = min(t.vpr[l], (n + V - 1) / V - v0);
     const T* zl = z + r * ld + t.start[l];
@@ -312,40 +403,39 @@ __global__ __launch_bounds__(256) void path_grad_kernel(const T* __restrict__ z,
     if (lane < t.G) {
       const int64_t e = (r * t.G + lane) * t.L + l;
       y = paths[e];
+      const float ce = coef[e];
       if (y < 0) y = -1;
-      else c = coef[e] * scale;
-      if (y >= n) c = __builtin_nanf("");
+      else c = y < n ? ce * scale : __builtin_nanf("");
     }
     const float A = group_sum<64>(c);
+    const bool live = A != 0.0f;                                                  // (true for NaN)
     float k = 0.0f, m = 0.0f;
     Run<T> run;
-    if (A != 0.0f) {                                                              // (true for NaN)
+    if (live) {
       run.load(zl, v0, nv, n, lane);
-      const float2 ms = merge_runs(partials + r * t.S + t.first[l], t.first[l + 1] - t.first[l]);
-      m = ms.x; k = -A / ms.y;
-#pragma unroll
-      for (int j = 0; j < NL; ++j)
-#pragma unroll
-        for (int e = 0; e < V; ++e) run.x[j][e] = k * fast_exp(run.x[j][e] - m);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NL; ++j)
-#pragma unroll
-        for (int e = 0; e < V; ++e) run.x[j][e] = 0.0f;
+      const float2 ms = merge_runs_wave(partials + r * t.S + t.first[l], t.first[l + 1] - t.first[l], lane);
+      k = -A / ms.y; m = ms.x;
     }
+    const bool mine = y >= (int64_t)v0 * V && y < (int64_t)(v0 + nv) * V && y < n;
+    const bool named = __ballot(mine) != 0;                                       // a path names a class of this run
+    float zy = 0.0f;
+    if (live && mine) zy = Elt<T>::load(zl + y);
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int i = j * 64 + lane, e0 = (v0 + i) * V;
+      if (j * 64 >= nv) break;
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = live ? k * fast_exp(run.get(j, e) - m) : 0.0f;
       if (i < nv) {
-        if (e0 + V <= n) store16(gl + e0, Elt<T>::pack(run.x[j]));
+        if (e0 + V <= n) store16(gl + e0, Elt<T>::pack(f));
         else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) if (e0 + e < n) gl[e0 + e] = Elt<T>::cvt(run.x[j][e]);
+          for (int e = 0; e < V; ++e) if (e0 + e < n) gl[e0 + e] = Elt<T>::cvt(f[e]);
         }
       }
     }
-    const bool mine = y >= (int64_t)v0 * V && y < (int64_t)(v0 + nv) * V && y < n;
-    if (__ballot(mine)) {
+    if (named) {
       float tot = 0.0f;
       bool leader = mine;
       for (int g = 0; g < t.G; ++g) {
@@ -353,8 +443,7 @@ __global__ __launch_bounds__(256) void path_grad_kernel(const T* __restrict__ z,
         const float cg = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), g));
         if (yg == (int)y) { tot += cg; if (g < lane) leader = false; }
       }
-      float soft = 0.0f;
-      if (leader && A != 0.0f) soft = k * fast_exp(Elt<T>::load(zl + y) - m);
+      const float soft = live ? k * fast_exp(zy - m) : 0.0f;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                            // the vector stores above are in the cache before the same bytes are written again
       if (leader) gl[y] = Elt<T>::cvt(tot + soft);
     }
@@ -375,14 +464,15 @@ static int build_table(PathTable& t, const int32_t* sizes, int L, int C, int G, 
   }
   if (s != C) { set_error("path loss: level sizes sum to %lld or more, expected C=%d", (long long)s, C); return LEC_E_ARG; }
   t.S = t.first[L];
+  t.byS = make_fastdiv(t.S); t.byG = make_fastdiv(G);
   return LEC_OK;
 }
 
 static int64_t wave_grid(int64_t waves) { const int64_t b = (waves + 3) / 4; return b > (1 << 22) ? (1 << 22) : b; }
 constexpr int64_t kMaxSumBlocks = 2048;
 
-// workspace: [0, 256) the arrival counter | block sums (2048 x 4 doubles)
-constexpr int64_t kWorkBytes = 256 + kMaxSumBlocks * 4 * 8;
+// workspace: the arrival counters, 33 lines of 128 bytes | block sums (2048 x 4 doubles)
+constexpr int64_t kCounterBytes = 33 * 128, kWorkBytes = kCounterBytes + kMaxSumBlocks * 4 * 8;
 
 template <typename F> static int by_type(int dtype, F&& f) {
   switch (dtype) {
@@ -401,10 +491,10 @@ static int table_for(PathTable& t, int dtype, int64_t R, int C, const int32_t* s
   return dtype == LEC_DTYPE_F32 ? build_table(t, sizes, L, C, G, Elt<float>::V, Elt<float>::NL) : build_table(t, sizes, L, C, G, Elt<_Float16>::V, Elt<_Float16>::NL);
 }
 
-static int run_stats(const void* z, int dtype, int64_t ld, int64_t R, const PathTable& t, float2* partials, unsigned int* counter, hipStream_t st) {
+static int run_stats(const void* z, int dtype, int64_t ld, int64_t R, const PathTable& t, float2* partials, unsigned int* counters, hipStream_t st) {
   const int rc = by_type(dtype, [&](auto* tag) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
-    hipLaunchKernelGGL((path_stats_kernel<T>), dim3((unsigned)wave_grid(R * t.S)), dim3(256), 0, st, (const T*)z, ld, R, t, partials, counter);
+    hipLaunchKernelGGL((path_stats_kernel<T>), dim3((unsigned)wave_grid(R * t.S)), dim3(256), 0, st, (const T*)z, ld, R, t, partials, counters);
   });
   if (rc != LEC_OK) return rc;
   LEC_CHECK_LAUNCH("path_stats_kernel");
@@ -469,14 +559,16 @@ extern "C" int lec_preference_loss_fwd(const void* logits, int dtype, int64_t ld
   LEC_CHECK_ARG(workspace && workspace_bytes >= kWorkBytes, "preference_loss: workspace needs %lld bytes", (long long)kWorkBytes);
   LEC_CHECK_ARG(label_smoothing >= 0.0f && label_smoothing <= 1.0f, "preference_loss: label_smoothing %g is not in [0, 1]", (double)label_smoothing);
   hipStream_t st = (hipStream_t)stream;
-  unsigned int* counter = (unsigned int*)workspace;
-  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, counter, st);
+  unsigned int* counters = (unsigned int*)workspace;
+  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, counters, st);
   if (rs != LEC_OK) return rs;
-  const int64_t blocks = (P + 7) / 8;
+  int LW = 1;
+  while (LW < L) LW <<= 1;
+  const int64_t per = 128 / LW, blocks = (P + per - 1) / per;
   by_type(dtype, [&](auto* tag) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
-    hipLaunchKernelGGL((preference_kernel<T>), dim3((unsigned)(blocks > kMaxSumBlocks ? kMaxSumBlocks : blocks)), dim3(256), 0, st, (const T*)logits, ld, P, shared, t, paths, ref,
-                       beta, label_smoothing, (const float2*)partials, coef, rewards, loss, (double*)((char*)workspace + 256), counter);
+    hipLaunchKernelGGL((preference_kernel<T>), dim3((unsigned)(blocks > kMaxSumBlocks ? kMaxSumBlocks : blocks)), dim3(256), 0, st, (const T*)logits, ld, P, shared, LW, t, paths, ref,
+                       beta, label_smoothing, (const float2*)partials, coef, rewards, loss, (double*)((char*)workspace + kCounterBytes), counters);
   });
   LEC_CHECK_LAUNCH("preference_kernel");
   return LEC_OK;
@@ -494,8 +586,8 @@ extern "C" int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, in
   LEC_CHECK_ARG(clip_low >= 0.0f && clip_high >= 0.0f, "policy_loss: clip bounds %g, %g are negative", (double)clip_low, (double)clip_high);
   LEC_CHECK_ARG(kl_coef == 0.0f || ref_logp, "policy_loss: a KL coefficient needs the reference's log-probabilities");
   hipStream_t st = (hipStream_t)stream;
-  unsigned int* counter = (unsigned int*)workspace;
-  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, counter, st);
+  unsigned int* counters = (unsigned int*)workspace;
+  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, counters, st);
   if (rs != LEC_OK) return rs;
   int LW = 1;
   while (LW < L) LW <<= 1;
@@ -503,7 +595,7 @@ extern "C" int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, in
   by_type(dtype, [&](auto* tag) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
     hipLaunchKernelGGL((policy_kernel<T>), dim3((unsigned)(blocks > kMaxSumBlocks ? kMaxSumBlocks : blocks)), dim3(256), 0, st, (const T*)logits, ld, n, LW, t, paths, adv, old_logp,
-                       ref_logp, clip_low, clip_high, kl_coef, per_path, (const float2*)partials, coef, loss, stats, norm, (double*)((char*)workspace + 256), counter);
+                       ref_logp, clip_low, clip_high, kl_coef, per_path, (const float2*)partials, coef, loss, stats, norm, (double*)((char*)workspace + kCounterBytes), counters);
   });
   LEC_CHECK_LAUNCH("policy_kernel");
   return LEC_OK;
