@@ -85,15 +85,27 @@ template <> struct Elt<_Float16> {
 
 // 16 bytes at element alignment (the compiler emits one dwordx4 access: the target's unaligned access mode)
 template <typename T> __device__ __forceinline__ uint4 load16(const T* p) { uint4 w; __builtin_memcpy(&w, (const void*)p, 16); return w; }
-#ifdef V_NT
-typedef unsigned int u32x4s __attribute__((ext_vector_type(4)));
-typedef u32x4s u32x4s_at2 __attribute__((aligned(2)));
-template <typename T> __device__ __forceinline__ void store16(T* p, const uint4& w) { __builtin_nontemporal_store(u32x4s{w.x, w.y, w.z, w.w}, (u32x4s_at2*)p); }
-#else
 template <typename T> __device__ __forceinline__ void store16(T* p, const uint4& w) { __builtin_memcpy((void*)p, &w, 16); }
-#endif
 
-__device__ __forceinline__ float fast_exp(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }      // t <= 0: absolute error of a softmax term below 2^-23
+// exp(t) for t <= 0 by the base-2 instruction: relative error below (3 |t| + 2) 2^-24
+__device__ __forceinline__ float fast_exp(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }
+
+// exp(x - m) for many x and one m, times a constant: one fma and one exponential an element.  x log2e - M, M = fl(m log2e), is exact but for its own rounding; what M lacks,
+// r = m log2e - M (exact in one fma), is the same for all and goes into the constant: exp(x - m) = 2^(x log2e - M) 2^-r.  Where m log2e leaves the floats' range (a level full
+// of the type's lowest value) the difference is taken first.  m = -inf (nothing finite): every term is exp(-inf) = 0.
+struct ExpAt {
+  float m, M, unit;                                              // unit = 2^-r
+  bool plain;
+  __device__ __forceinline__ explicit ExpAt(float top) {
+    m = top == -INFINITY ? 0.0f : top;
+    plain = fabsf(m) < 1e38f;                                    // (the same in all lanes: the branch below is scalar)
+    M = m * kLog2e;
+    unit = plain ? __builtin_amdgcn_exp2f(-__builtin_fmaf(m, kLog2e, -M)) : 1.0f;
+  }
+  template <bool PLAIN> __device__ __forceinline__ float at(float x) const {      // times unit
+    return PLAIN ? __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, -M)) : fast_exp(x - m);
+  }
+};
 
 // One run of a level of n elements at z: vectors v0 .. v0 + nv, one in 64 a lane, raw; -inf where there is none.
 template <typename T>
@@ -144,15 +156,18 @@ __global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z
 #pragma unroll
       for (int e = 0; e < V; ++e) m = fmaxf(m, run.get(j, e));
     m = group_max<64>(m);
-    const float mm = m == -INFINITY ? 0.0f : m;                                  // nothing finite: the terms are exp(-inf) = 0 (NaN stays NaN)
+    const ExpAt ex(m);
     float s = 0.0f;
+    auto sum = [&](auto plain) {
 #pragma unroll
-    for (int j = 0; j < NL; ++j)
-      if (j * 64 < nv) {
+      for (int j = 0; j < NL; ++j)
+        if (j * 64 < nv) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += fast_exp(run.get(j, e) - mm);
-      }
-    s = group_sum<64>(s);
+          for (int e = 0; e < V; ++e) s += ex.template at<decltype(plain)::value>(run.get(j, e));
+        }
+    };
+    if (ex.plain) sum(std::true_type{}); else sum(std::false_type{});
+    s = group_sum<64>(s) * ex.unit;
     if (lane == 0) partials[task] = make_float2(m, s);
   }
 }
@@ -409,32 +424,38 @@ __global__ __launch_bounds__(256) void path_grad_kernel(const T* __restrict__ z,
     }
     const float A = group_sum<64>(c);
     const bool live = A != 0.0f;                                                  // (true for NaN)
-    float k = 0.0f, m = 0.0f;
+    float2 ms = make_float2(0.0f, 1.0f);
     Run<T> run;
     if (live) {
       run.load(zl, v0, nv, n, lane);
-      const float2 ms = merge_runs_wave(partials + r * t.S + t.first[l], t.first[l + 1] - t.first[l], lane);
-      k = -A / ms.y; m = ms.x;
+      ms = merge_runs_wave(partials + r * t.S + t.first[l], t.first[l + 1] - t.first[l], lane);
     }
+    const ExpAt ex(ms.x);
+    const float k = -A / ms.y * ex.unit;
     const bool mine = y >= (int64_t)v0 * V && y < (int64_t)(v0 + nv) * V && y < n;
     const bool named = __ballot(mine) != 0;                                       // a path names a class of this run
     float zy = 0.0f;
     if (live && mine) zy = Elt<T>::load(zl + y);
+    auto write = [&](auto value) {
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int i = j * 64 + lane, e0 = (v0 + i) * V;
-      if (j * 64 >= nv) break;
-      float f[V];
+      for (int j = 0; j < NL; ++j) {
+        const int i = j * 64 + lane, e0 = (v0 + i) * V;
+        if (j * 64 >= nv) break;
+        float f[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = live ? k * fast_exp(run.get(j, e) - m) : 0.0f;
-      if (i < nv) {
-        if (e0 + V <= n) store16(gl + e0, Elt<T>::pack(f));
-        else {
+        for (int e = 0; e < V; ++e) f[e] = value(j, e);
+        if (i < nv) {
+          if (e0 + V <= n) store16(gl + e0, Elt<T>::pack(f));
+          else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) if (e0 + e < n) gl[e0 + e] = Elt<T>::cvt(f[e]);
+            for (int e = 0; e < V; ++e) if (e0 + e < n) gl[e0 + e] = Elt<T>::cvt(f[e]);
+          }
         }
       }
-    }
+    };
+    if (!live) write([&](int, int) { return 0.0f; });
+    else if (ex.plain) write([&](int j, int e) { return k * ex.template at<true>(run.get(j, e)); });
+    else write([&](int j, int e) { return k * ex.template at<false>(run.get(j, e)); });
     if (named) {
       float tot = 0.0f;
       bool leader = mine;
@@ -443,7 +464,7 @@ __global__ __launch_bounds__(256) void path_grad_kernel(const T* __restrict__ z,
         const float cg = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), g));
         if (yg == (int)y) { tot += cg; if (g < lane) leader = false; }
       }
-      const float soft = live ? k * fast_exp(zy - m) : 0.0f;
+      const float soft = !live ? 0.0f : k * (ex.plain ? ex.template at<true>(zy) : ex.template at<false>(zy));
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                            // the vector stores above are in the cache before the same bytes are written again
       if (leader) gl[y] = Elt<T>::cvt(tot + soft);
     }

@@ -214,6 +214,23 @@ def test_excluded_classes_and_special_values():
 
 
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+def test_levels_full_of_the_lowest_or_highest_value_are_uniform(dtype):
+    """Every class at the type's lowest (highest) value: the softmax is uniform; one class apart from the rest takes it all.  Offsets that no difference shows change nothing."""
+    from learning_embeddings_amd import loss
+    lv = [4, 700, 3000]
+    f = torch.finfo(DT[dtype])
+    z = torch.zeros(4, 3704, dtype=DT[dtype])
+    z[0] = f.min; z[1] = f.max; z[2] = f.min; z[2, 4:8] = 0.0; z[3] = 1000.0
+    paths = np.full((4, 1, 3), 2, dtype=np.int64)
+    zt = dev(z).requires_grad_()
+    lp = loss.path_log_probs(zt, dev(paths), lv)
+    lp.backward(torch.ones_like(lp))
+    want = -np.log(np.array([[4, 700, 3000], [4, 700, 3000], [4, 4, 3000], [4, 700, 3000]], dtype=np.float64))
+    assert (np.abs(lp.detach().cpu().numpy()[:, 0] - want) <= LT(lv) + U * np.abs(want)).all()
+    check_grad(zt.grad, z, z.double().numpy(), paths, lv, np.ones(paths.shape), np.full(paths.shape, 2 * U), dtype)
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
 def test_strided_transposed_and_broadcast_logits(dtype):
     from learning_embeddings_amd import loss
     lv = [3, 5, 600]
