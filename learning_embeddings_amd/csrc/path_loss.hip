@@ -138,8 +138,10 @@ __device__ __forceinline__ int level_of(const PathTable& t, int slot) {
   return l;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z, int64_t ld, int64_t R, PathTable t, float2* __restrict__ partials, unsigned int* counters) {
+// LOGP: every level is one run, and the wave writes its entries' log-probabilities too.
+template <typename T, bool LOGP>
+__global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z, int64_t ld, int64_t R, PathTable t, float2* __restrict__ partials, unsigned int* counters,
+                                                         const int64_t* __restrict__ paths, float* __restrict__ logp) {
   const int lane = threadIdx.x & 63;
   if (counters && blockIdx.x == 0 && threadIdx.x <= 32) counters[threadIdx.x * 32] = 0;      // armed for the loss kernel behind this launch (grid_sum)
   const int64_t ntask = R * t.S, nwave = (int64_t)gridDim.x * 4;
@@ -148,8 +150,13 @@ __global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z
     const int slot = (int)(task - r * t.S), l = level_of(t, slot), n = t.start[l + 1] - t.start[l];
     constexpr int V = Elt<T>::V, NL = Elt<T>::NL;
     const int v0 = (slot - t.first[l]) * t.vpr[l], nv = min(t.vpr[l], (n + V - 1) / V - v0);
+    const T* zl = z + r * ld + t.start[l];
+    const int64_t entry = (r * t.G + lane) * t.L + l;
+    int64_t y = -1;
+    if (LOGP && lane < t.G) y = paths[entry];
     Run<T> run;
-    run.load(z + r * ld + t.start[l], v0, nv, n, lane);
+    run.load(zl, v0, nv, n, lane);
+    const float zy = LOGP && y >= 0 && y < n ? Elt<T>::load(zl + y) : __builtin_nanf("");
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NL; ++j)
@@ -169,6 +176,7 @@ __global__ __launch_bounds__(256) void path_stats_kernel(const T* __restrict__ z
     if (ex.plain) sum(std::true_type{}); else sum(std::false_type{});
     s = group_sum<64>(s) * ex.unit;
     if (lane == 0) partials[task] = make_float2(m, s);
+    if (LOGP && lane < t.G) logp[entry] = y < 0 ? 0.0f : (float)(((double)zy - (double)m) - log((double)s));
   }
 }
 
@@ -512,10 +520,12 @@ static int table_for(PathTable& t, int dtype, int64_t R, int C, const int32_t* s
   return dtype == LEC_DTYPE_F32 ? build_table(t, sizes, L, C, G, Elt<float>::V, Elt<float>::NL) : build_table(t, sizes, L, C, G, Elt<_Float16>::V, Elt<_Float16>::NL);
 }
 
-static int run_stats(const void* z, int dtype, int64_t ld, int64_t R, const PathTable& t, float2* partials, unsigned int* counters, hipStream_t st) {
+static int run_stats(const void* z, int dtype, int64_t ld, int64_t R, const PathTable& t, float2* partials, unsigned int* counters, hipStream_t st, const int64_t* paths = nullptr,
+                     float* logp = nullptr) {
   const int rc = by_type(dtype, [&](auto* tag) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
-    hipLaunchKernelGGL((path_stats_kernel<T>), dim3((unsigned)wave_grid(R * t.S)), dim3(256), 0, st, (const T*)z, ld, R, t, partials, counters);
+    const auto kernel = logp ? path_stats_kernel<T, true> : path_stats_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wave_grid(R * t.S)), dim3(256), 0, st, (const T*)z, ld, R, t, partials, counters, paths, logp);
   });
   if (rc != LEC_OK) return rc;
   LEC_CHECK_LAUNCH("path_stats_kernel");
@@ -541,8 +551,9 @@ extern "C" int lec_path_logp_fwd(const void* logits, int dtype, int64_t ld, int6
   if (rc != LEC_OK) return rc;
   LEC_CHECK_ARG(R > 0 && logits && paths && logp && partials && ld >= C, "path_logp_fwd: null pointer or ld=%lld < C=%d or no rows", (long long)ld, C);
   hipStream_t st = (hipStream_t)stream;
-  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, nullptr, st);
-  if (rs != LEC_OK) return rs;
+  const bool one_launch = t.S == t.L;                            // every level fits one wave's run: the wave that has its sum also has what its entries need
+  const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, nullptr, st, paths, one_launch ? logp : nullptr);
+  if (rs != LEC_OK || one_launch) return rs;
   const int64_t n = R * G * L, blocks = (n + 255) / 256;
   by_type(dtype, [&](auto* tag) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;

@@ -9,6 +9,8 @@ import torch
 import torch.nn as nn
 
 from . import parallel
+from .loss import path_log_probs
+from .quant import MXFP4Linear
 from .resnet import resnet18, resnet50
 
 
@@ -159,3 +161,61 @@ class ETHECExperiment(Experiment):
         if loss.is_cuda:
             done = torch.cuda.Event(); done.record(); pend.append(done)
         return loss, outputs
+
+    # ---- learning from feedback on the model's answers (label paths) instead of labels; no counterpart in the reference
+    def freeze_reference(self, head='mxfp4'):
+        """Keeps a frozen copy of the present model as `self.reference` -- what the preference loss and the KL term measure against.  head: 'mxfp4' holds the classifier
+        in 4 bits (a quarter of bf16's weights; its log-probabilities are close to, not equal to, the model's), 'full' keeps it as it is."""
+        if head not in ('mxfp4', 'full'):
+            raise ValueError("head must be 'mxfp4' or 'full', got %r" % (head,))
+        ref = copy.deepcopy(self.model)
+        for p in ref.parameters():
+            p.requires_grad = False
+        ref.wgrad_overlap = False
+        if head == 'mxfp4':
+            ref.fc = MXFP4Linear.from_linear(ref.fc, out_dtype=torch.float32)
+        self.reference = ref.eval()
+        return self.reference
+
+    def reference_log_probs(self, inputs, paths):
+        """Log-probabilities of paths ([B, L] or [B, G, L], see loss.path_log_probs) under the frozen reference."""
+        if getattr(self, 'reference', None) is None:
+            raise RuntimeError('no reference model: call freeze_reference() first')
+        with torch.no_grad(), torch.autocast('cuda', dtype=self.compute_dtype, enabled=self.compute_dtype != torch.float32):
+            outputs = self.reference(inputs.to(self.device, non_blocking=True).contiguous(memory_format=torch.channels_last))
+        return path_log_probs(outputs, paths.to(self.device), self.labelmap)
+
+    def preference_step(self, inputs, paths, criterion, ref_log_probs=None):
+        """One training step on preferences: criterion = loss.PreferenceLoss, paths [B, 2, L] (two answers for every image, the preferred first) or, for 2P images of which the
+        first P carry the preferred answers, [2P, L].  ref_log_probs None: the frozen reference's.  -> (loss, rewards [P, 2])"""
+        inputs, paths = inputs.to(self.device, non_blocking=True), paths.to(self.device)
+        ref = self.reference_log_probs(inputs, paths) if ref_log_probs is None else ref_log_probs.to(self.device)
+        return self._feedback_step(inputs, lambda outputs: criterion(outputs, paths, ref))
+
+    def policy_step(self, inputs, paths, advantages, criterion, old_log_probs=None, ref_log_probs=None):
+        """One training step on rewards of sampled paths: criterion = loss.ClippedPolicyLoss, paths [B, G, L] or [B, L], advantages [B, G] or [B].  ref_log_probs None: the
+        frozen reference's where the criterion has a KL term.  -> (loss, stats [2])"""
+        inputs, paths = inputs.to(self.device, non_blocking=True), paths.to(self.device)
+        if ref_log_probs is None and criterion.kl_coef != 0.0:
+            ref_log_probs = self.reference_log_probs(inputs, paths)
+        at = lambda t: None if t is None else t.to(self.device)
+        adv, old, ref = at(advantages), at(old_log_probs), at(ref_log_probs)
+        return self._feedback_step(inputs, lambda outputs: criterion(outputs, paths, adv, old, ref))
+
+    def _feedback_step(self, inputs, criterion):
+        """train_step with a criterion of the outputs alone that returns (loss, what it reports); the mean is over the LOCAL batch, as there."""
+        pend = self.__dict__.setdefault('_steps_in_flight', [])
+        if len(pend) >= 2:
+            pend.pop(0).synchronize()
+        inputs = inputs.to(self.device, non_blocking=True).contiguous(memory_format=torch.channels_last)
+        self.arena.zero_grad()
+        with torch.autocast('cuda', dtype=self.compute_dtype, enabled=self.compute_dtype != torch.float32):
+            outputs = self.model(inputs)
+        loss, report = criterion(outputs)
+        loss.backward()
+        if self.overlap is not None:
+            self.overlap.join()
+        self.reducer.finish()
+        self.arena.adam_step(self.lr, grad_scale=1.0 / self.world)
+        done = torch.cuda.Event(); done.record(); pend.append(done)
+        return loss.detach(), report

@@ -398,34 +398,44 @@ def _entries_arg(t, name, shape, like):
     return t.detach().to(torch.float32).contiguous()
 
 
-def _f32(g):
-    return g if g.dtype == torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
-
-
 def on_device_of(first):
     """Decorator of a function whose argument number `first` is a tensor: runs it with that tensor's device current (kernels are launched on, and buffers taken from, the
     current device)."""
     def deco(f):
-        def wrapped(*args):
+        def wrapped(*args, **kwargs):
             dev = args[first].device
             if dev.type != 'cuda' or dev.index == torch.cuda.current_device():
-                return f(*args)
+                return f(*args, **kwargs)
             with torch.cuda.device(dev):
-                return f(*args)
+                return f(*args, **kwargs)
         return wrapped
     return deco
 
 
 # Every buffer below belongs to the call (to its autograd node when a backward follows), so calls on other streams and captured graphs share nothing.
-# buf = [workspace | partials], see include/lecone.h.
+# buf = [workspace | partials | norm, 3 unused words | coefficients], see include/lecone.h.
+
+def _path_buffer(levels, code, R, entries, device):
+    """(buf, address of the workspace, of the partials, of norm)"""
+    part = levels.work
+    norm = part + R * levels.row_bytes[code]
+    buf = torch.empty(norm + 16 + 4 * entries, dtype=torch.uint8, device=device)
+    p = buf.data_ptr()
+    return buf, p, p + part, p + norm
+
 
 @on_device_of(1)
-def _path_backward(ctx, coef, coef_ptr, up, norm):
-    z, paths, buf = ctx.saved_tensors[:3]
+def _path_backward(ctx, gl, coef=None, has_norm=False):
+    """gl: the upstream gradient of a loss, or with coef = gl that of every entry."""
+    z, paths, buf = ctx.saved_tensors
     levels, code, ld, R, G = ctx.meta
+    part = buf.data_ptr() + levels.work
+    norm = part + R * levels.row_bytes[code]
+    gl = gl if gl.dtype == torch.float32 and gl.is_contiguous() else gl.to(torch.float32).contiguous()
+    coef_ptr, up = (norm + 16, gl.data_ptr()) if coef is None else (gl.data_ptr(), None)
     dz = torch.empty((R, levels.C), dtype=z.dtype, device=z.device)
-    check(lib.lec_path_logp_bwd(z.data_ptr(), code, ld, R, levels.C, levels.ptr, levels.L, paths.data_ptr(), G, buf.data_ptr() + levels.work, coef_ptr,
-                                up if up is None else up.data_ptr(), norm, dz.data_ptr(), levels.C, raw_stream(z.device.index)))
+    check(lib.lec_path_logp_bwd(z.data_ptr(), code, ld, R, levels.C, levels.ptr, levels.L, paths.data_ptr(), G, part, coef_ptr, up, norm if has_norm else None,
+                                dz.data_ptr(), levels.C, raw_stream(z.device.index)))
     return dz
 
 
@@ -442,9 +452,8 @@ class PathLogProbFn(torch.autograd.Function):
         if R == 0 or G == 0:
             ctx.empty = (tuple(logits.shape), logits.dtype, logits.device)
             return logp
-        buf = torch.empty(levels.work + R * levels.row_bytes[code], dtype=torch.uint8, device=z.device)
-        check(lib.lec_path_logp_fwd(z.data_ptr(), code, ld, R, levels.C, levels.ptr, levels.L, paths.data_ptr(), G, logp.data_ptr(), buf.data_ptr() + levels.work,
-                                    raw_stream(z.device.index)))
+        buf, _, part, _ = _path_buffer(levels, code, R, 0, z.device)
+        check(lib.lec_path_logp_fwd(z.data_ptr(), code, ld, R, levels.C, levels.ptr, levels.L, paths.data_ptr(), G, logp.data_ptr(), part, raw_stream(z.device.index)))
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(z, paths, buf)
             ctx.meta = (levels, code, ld, R, G)
@@ -456,8 +465,7 @@ class PathLogProbFn(torch.autograd.Function):
         if ctx.meta is None:
             shape, dtype, device = ctx.empty
             return torch.zeros(shape, dtype=dtype, device=device), None, None
-        g = _f32(g)
-        return _path_backward(ctx, g, g.data_ptr(), None, None), None, None
+        return _path_backward(ctx, g, coef=g), None, None
 
 
 class PreferenceLossFn(torch.autograd.Function):
@@ -472,13 +480,11 @@ class PreferenceLossFn(torch.autograd.Function):
         P, G = (R, 2) if shared else (R // 2, 1)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         rewards = torch.empty((P, 2), dtype=torch.float32, device=dev)
-        coef = torch.empty(R * G * levels.L, dtype=torch.float32, device=dev)
-        buf = torch.empty(levels.work + R * levels.row_bytes[code], dtype=torch.uint8, device=dev)
-        ws = buf.data_ptr()
+        buf, ws, part, norm = _path_buffer(levels, code, R, R * G * levels.L, dev)
         check(lib.lec_preference_loss_fwd(z.data_ptr(), code, ld, P, int(shared), levels.C, levels.ptr, levels.L, paths.data_ptr(), ref.data_ptr(), beta, smoothing,
-                                          loss.data_ptr(), rewards.data_ptr(), coef.data_ptr(), ws + levels.work, ws, levels.work, raw_stream(dev.index)))
+                                          loss.data_ptr(), rewards.data_ptr(), norm + 16, part, ws, levels.work, raw_stream(dev.index)))
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(z, paths, buf, coef)
+            ctx.save_for_backward(z, paths, buf)
             ctx.meta = (levels, code, ld, R, G)
         ctx.mark_non_differentiable(rewards)
         return loss, rewards
@@ -486,8 +492,7 @@ class PreferenceLossFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gl, _gr):
-        coef = ctx.saved_tensors[3]
-        return _path_backward(ctx, coef, coef.data_ptr(), _f32(gl), None), None, None, None
+        return _path_backward(ctx, gl), None, None, None
 
 
 class PolicyLossFn(torch.autograd.Function):
@@ -502,14 +507,12 @@ class PolicyLossFn(torch.autograd.Function):
         dev = z.device
         loss = torch.empty((), dtype=torch.float32, device=dev)
         stats = torch.empty(2, dtype=torch.float32, device=dev)
-        coef = torch.empty(4 + R * G * levels.L, dtype=torch.float32, device=dev)                   # norm, 3 unused | coefficients
-        buf = torch.empty(levels.work + R * levels.row_bytes[code], dtype=torch.uint8, device=dev)
-        ws, norm = buf.data_ptr(), coef.data_ptr()
+        buf, ws, part, norm = _path_buffer(levels, code, R, R * G * levels.L, dev)
         check(lib.lec_policy_loss_fwd(z.data_ptr(), code, ld, R, levels.C, levels.ptr, levels.L, paths.data_ptr(), G, adv.data_ptr(), old if old is None else old.data_ptr(),
                                       ref if ref is None else ref.data_ptr(), low, high, kl, int(per_path), loss.data_ptr(), stats.data_ptr(), norm, norm + 16,
-                                      ws + levels.work, ws, levels.work, raw_stream(dev.index)))
+                                      part, ws, levels.work, raw_stream(dev.index)))
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(z, paths, buf, coef)
+            ctx.save_for_backward(z, paths, buf)
             ctx.meta = (levels, code, ld, R, G)
         ctx.mark_non_differentiable(stats)
         return loss, stats
@@ -517,9 +520,7 @@ class PolicyLossFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gl, _gs):
-        coef = ctx.saved_tensors[3]
-        norm = coef.data_ptr()
-        return _path_backward(ctx, coef, norm + 16, _f32(gl), norm), None, None, None, None, None
+        return _path_backward(ctx, gl, has_norm=True), None, None, None, None, None
 
 
 # ------------------------------------------------------------------------------------------------ per-model fusion records
