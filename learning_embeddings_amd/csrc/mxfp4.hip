@@ -289,6 +289,7 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_linear_small_kernel(const 
 // push the operands out of the L2) 460; without any stores 360, without stores and operand traffic 285, and the matrix cores alone, on random operands, which run at 6.1
 // PFLOP/s under their power limit, 250.
 constexpr int kBigTile = 192;
+constexpr int kBigLds = 4 * 96 * 208 + kBigTile * 4;             // the ring (72 KB) and, after it, the waves' output images in the same place; the block's biases
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 typedef __attribute__((address_space(3))) void lds_ptr;
@@ -346,8 +347,12 @@ __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ 
   };
   const uint4* A = (const uint4*)smem + wn * W * 128 + lane;     // this wave's operand tiles of slot 0: [W row tiles][2 k tiles]
   const uint4* B = (const uint4*)(smem + SIDE) + wm * W * 128 + lane;
+  float* s_bias = (float*)(smem + kBigLds - kBigTile * 4);                 // behind the ring and the image
+  const rsrc_t rbias = make_rsrc(bias, bias ? (unsigned)N * 4u : 0u);
+  const float bias_here = threadIdx.x < kBigTile ? bias_at(rbias, bn * kBigTile + (int)threadIdx.x) : 0.0f;      // (past the end: 0)
   fetch_scales(0);
   issue(0, 0); issue(1, 1); issue(2, 2);
+  if (threadIdx.x < kBigTile) s_bias[threadIdx.x] = bias_here;
   wait_vm<2 * IPW>();                                            // stage 0 has landed for this wave ...
   meet();                                                        // ... and for every wave
 #pragma unroll
@@ -402,7 +407,6 @@ __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ 
     for (int i = 0; i < W; ++i) { sa[i] = na[i]; sb[i] = nb[i]; }
   }
   wait_vm<0>();                                                  // (the stages of zeros past the end still write LDS)
-  const rsrc_t rbias = make_rsrc(bias, bias ? (unsigned)N * 4u : 0u);
   const bool inside = (int64_t)(bn + 1) * kBigTile <= N && (int64_t)(bm + 1) * kBigTile <= M;
   const int64_t m0 = (int64_t)bm * kBigTile + wm * 32 * W;
   const int n0 = bn * kBigTile + wn * 32 * W;
@@ -422,9 +426,9 @@ __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ 
           const int nn = i * 32 + 16 * h - part * CW;            // (16 classes lie in one half: CW is 96 or 48)
           if (nn < 0 || nn >= CW) continue;
           float bl[4], bh[4];
-          const int nl = n0 + i * 32 + 16 * h + 4 * (lane >> 5);
+          const float* pb = s_bias + wn * 32 * W + i * 32 + 16 * h + 4 * (lane >> 5);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { bl[e] = bias_at(rbias, nl + e); bh[e] = bias_at(rbias, nl + 8 + e); }
+          for (int e = 0; e < 4; ++e) { bl[e] = pb[e]; bh[e] = pb[8 + e]; }
 #pragma unroll
           for (int j = 0; j < W; ++j) {
             __attribute__((aligned(16))) T lo[4], hi[4];
@@ -558,9 +562,9 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
     int rl = LEC_OK;
     by_dtype(ydtype, "", [&](auto* tag) {
       using T = std::remove_pointer_t<decltype(tag)>;
-      static const hipError_t set = hipFuncSetAttribute((const void*)mxfp4_linear_big_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, 4 * 96 * 208);
+      static const hipError_t set = hipFuncSetAttribute((const void*)mxfp4_linear_big_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds);
       if (set != hipSuccess) { rl = hip_fail(set, "mxfp4_linear_big_kernel"); return; }
-      hipLaunchKernelGGL((mxfp4_linear_big_kernel<T>), dim3((unsigned)(per * 8)), dim3(256), 4 * 96 * 208, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
+      hipLaunchKernelGGL((mxfp4_linear_big_kernel<T>), dim3((unsigned)(per * 8)), dim3(256), kBigLds, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
                          (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy, (int)nbn, (int)nbm, (int)per);
     });
     if (rl != LEC_OK) return rl;
