@@ -13,6 +13,9 @@
 #include "lec_common.h"
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
+#include <mutex>
+#include <set>
+#include <utility>
 
 namespace lec {
 
@@ -181,27 +184,56 @@ __device__ __forceinline__ void store_tile(T* __restrict__ y, int64_t ldy, int64
   }
 }
 
-// At most 32 rows (one tile of x): the time is the weights' way from memory.  Two waves share a tile of 32 classes, each half of its k tiles (of a chunk of 32), all asked for
-// at once; while they are under way the block quantises x into LDS (each block again: x is small and comes from the L2, a launch of its own would cost more).  x has to fit
-// LDS beside the join: K <= 3 328.  Columns of x's tile that are no row of x are never written: a column of the product depends on its own column only, and those are not stored.
+// Two waves share a tile of 32 classes, each about half of its k tiles, in whole scale words: this wave's are [lo, hi).
+__device__ __forceinline__ void half_of(int KT, int half, int& lo, int& hi) {
+  const int mid = min((((KT + 1) >> 1) + 3) & ~3, KT);
+  lo = half ? mid : 0; hi = half ? KT : mid;
+}
+// Up to CH of a wave's weight tiles and their scale words, all asked for at once
+constexpr int CH = 16;
+struct WeightTiles {
+  uint4 w[CH];
+  unsigned int s[CH / 4];
+  __device__ __forceinline__ void fetch(const uint4* __restrict__ wc, const unsigned int* __restrict__ wsc, int64_t nt, int KT, int KG, int kt0, int hi, int lane) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) if (kt0 + i < hi) w[i] = wc[(nt * KT + kt0 + i) * 64 + lane];
+#pragma unroll
+    for (int i = 0; i < CH / 4; ++i) if (kt0 + 4 * i < hi) s[i] = wsc[(nt * KG + (kt0 >> 2) + i) * 64 + lane];
+  }
+};
+// The second half's sums, joined in a fixed order; true for the wave that then holds the whole of them.  All threads of the block call it.
+__device__ __forceinline__ bool join_halves(f32x16& acc, f32x4 (*s_half)[4][64], int pair, int half, int lane) {
+  if (half) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) s_half[pair][g][lane] = f32x4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+  }
+  __syncthreads();
+  if (half) return false;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 o = s_half[pair][g][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[4 * g + e] += o[e];
+  }
+  return true;
+}
+
+// A few rows: the time is the weights' way from memory, and a launch to quantise x would cost more than x is worth, so every block quantises it into LDS while its weights
+// are under way.  x has to fit LDS beside the join: K <= 3 328.  Columns of x's tile that are no row of x are never written: a column of the product depends on its own
+// column only, and those are not stored.
 template <typename TX, typename T>
-__global__ __launch_bounds__(256) void mxfp4_linear_rows_kernel(const TX* __restrict__ x, int64_t ldx, int M, const uint4* __restrict__ wc, const unsigned int* __restrict__ wsc, int N, int K,
-                                                                int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy) {
+__global__ __launch_bounds__(256) void mxfp4_linear_few_kernel(const TX* __restrict__ x, int64_t ldx, int M, const uint4* __restrict__ wc, const unsigned int* __restrict__ wsc, int N, int K,
+                                                               int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ f32x4 s_half[2][4][64];
   unsigned int* xcodes = (unsigned int*)smem;                    // [KT][64][4] words
   unsigned char* xscale = smem + (size_t)KT * 1024;              // [KG][64][4] bytes
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = wave & 1;
   const int ntn = (N + 31) >> 5, nt_ = (int)blockIdx.x * 2 + (wave >> 1), nt = min(nt_, ntn - 1);        // (a pair past the last tile repeats it and stores nothing)
-  constexpr int CH = 16;
-  uint4 w[CH];
-  unsigned int sw[CH / 4];
-  auto fetch = [&](int kt0) {                                    // this wave's tiles of the chunk: kt0 + 16 half .. + 16
-#pragma unroll
-    for (int i = 0; i < CH; ++i) if (kt0 + CH * half + i < KT) w[i] = wc[((int64_t)nt * KT + kt0 + CH * half + i) * 64 + lane];
-#pragma unroll
-    for (int i = 0; i < CH / 4; ++i) if (kt0 / 4 + CH / 4 * half + i < KG) sw[i] = wsc[((int64_t)nt * KG + kt0 / 4 + CH / 4 * half + i) * 64 + lane];
-  };
-  fetch(0);
+  int lo, hi;
+  half_of(KT, half, lo, hi);
+  WeightTiles W;
+  W.fetch(wc, wsc, nt, KT, KG, lo, hi, lane);
   const int per_row = KG * 32;                                   // 8-element pieces of a row, padded to whole groups of 256
   for (int i = t; i < M * per_row; i += 256) {
     const int r = i / per_row, q = i - r * per_row, k = q * 8, kt = k >> 6, kh = (k >> 5) & 1, sub = (k >> 3) & 3;
@@ -214,70 +246,44 @@ __global__ __launch_bounds__(256) void mxfp4_linear_rows_kernel(const TX* __rest
   }
   __syncthreads();
   f32x16 acc = zero16();
-  for (int kt0 = 0; kt0 < KT; kt0 += 2 * CH) {
-    if (kt0) fetch(kt0);
+  for (int kt0 = lo; kt0 < hi; kt0 += CH) {
+    if (kt0 > lo) W.fetch(wc, wsc, nt, KT, KG, kt0, hi, lane);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int kt = kt0 + CH * half + i;
-      if (kt < KT) acc = mfma4(w[i], ((const uint4*)xcodes)[kt * 64 + lane], acc, i & 3, sw[i >> 2], ((const unsigned int*)xscale)[(kt >> 2) * 64 + lane]);
+      const int kt = kt0 + i;
+      if (kt < hi) acc = mfma4(W.w[i], ((const uint4*)xcodes)[kt * 64 + lane], acc, i & 3, W.s[i >> 2], ((const unsigned int*)xscale)[(kt >> 2) * 64 + lane]);
     }
   }
-  __shared__ f32x4 s_half[2][4][64];                             // the second half's sums, joined in a fixed order
-  if (half) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) s_half[wave >> 1][g][lane] = f32x4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
-  }
-  __syncthreads();
-  if (half || nt_ != nt) return;
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const f32x4 o = s_half[wave >> 1][g][lane];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[4 * g + e] += o[e];
-  }
-  store_tile(y, ldy, M, N, 0, nt * 32, lane, make_rsrc(bias, bias ? (unsigned)N * 4u : 0u), acc);
+  if (join_halves(acc, s_half, wave >> 1, half, lane) && nt_ == nt) store_tile(y, ldy, M, N, 0, nt * 32, lane, make_rsrc(bias, bias ? (unsigned)N * 4u : 0u), acc);
 }
 
-// A block of WN x WM waves, a wave NT x MT tiles, operands straight from memory (every load is a contiguous kilobyte): few tiles, or shapes too small for the ring below.
-template <typename T, int WN, int WM, int NT, int MT>
-__global__ __launch_bounds__(64 * WN * WM) void mxfp4_linear_small_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
-                                                                          const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y,
-                                                                          int64_t ldy) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nt0 = ((int)blockIdx.x * WN + wave % WN) * NT, ntn = (N + 31) >> 5;
-  const int64_t mt0 = ((int64_t)blockIdx.y * WM + wave / WN) * MT, mtn = (M + 31) >> 5;
-  if (nt0 >= ntn || mt0 >= mtn) return;
-  f32x16 acc[NT][MT];
+// Up to 32 rows, and products too small for the ring below: a wave pair a tile of 32 classes x 32 rows, the weights asked for all at once, x (in 4 bits, from the L2) four k
+// tiles at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void mxfp4_linear_rows_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
+                                                                const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy) {
+  __shared__ f32x4 s_half[2][4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave & 1;
+  const int ntn = (N + 31) >> 5, nt_ = (int)blockIdx.x * 2 + (wave >> 1), nt = min(nt_, ntn - 1);        // (a pair past the last tile repeats it and stores nothing)
+  const int64_t mt = blockIdx.y;
+  int lo, hi;
+  half_of(KT, half, lo, hi);
+  f32x16 acc = zero16();
+  WeightTiles W;
+  for (int kt0 = lo; kt0 < hi; kt0 += CH) {
+    W.fetch(wc, wsc, nt, KT, KG, kt0, hi, lane);
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+    for (int h = 0; h < CH / 4; ++h) {
+      if (kt0 + 4 * h >= hi) break;
+      uint4 b[4];
+      const unsigned int sb = xs[(mt * KG + (kt0 >> 2) + h) * 64 + lane];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = zero16();
-  for (int kg = 0; kg < KG; ++kg) {
-    unsigned int sa[NT], sb[MT];
+      for (int i = 0; i < 4; ++i) if (kt0 + 4 * h + i < hi) b[i] = xc[(mt * KT + kt0 + 4 * h + i) * 64 + lane];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) sa[i] = wsc[((int64_t)min(nt0 + i, ntn - 1) * KG + kg) * 64 + lane];       // (tiles past the end repeat the last one; they are not stored)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) sb[j] = xs[(min(mt0 + j, mtn - 1) * KG + kg) * 64 + lane];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int kt = kg * 4 + q;
-      if (kt >= KT) break;
-      uint4 a[NT], b[MT];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) a[i] = wc[((int64_t)min(nt0 + i, ntn - 1) * KT + kt) * 64 + lane];
-#pragma unroll
-      for (int j = 0; j < MT; ++j) b[j] = xc[(min(mt0 + j, mtn - 1) * KT + kt) * 64 + lane];
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = mfma4(a[i], b[j], acc[i][j], q, sa[i], sb[j]);
+      for (int i = 0; i < 4; ++i) if (kt0 + 4 * h + i < hi) acc = mfma4(W.w[4 * h + i], b[i], acc, i, W.s[h], sb);
     }
   }
-  const rsrc_t rbias = make_rsrc(bias, bias ? (unsigned)N * 4u : 0u);
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) store_tile(y, ldy, M, N, (mt0 + j) * 32, (nt0 + i) * 32, lane, rbias, acc[i][j]);
+  if (join_halves(acc, s_half, wave >> 1, half, lane) && nt_ == nt) store_tile(y, ldy, M, N, mt * 32, nt * 32, lane, make_rsrc(bias, bias ? (unsigned)N * 4u : 0u), acc);
 }
 
 // Large products.  A block of 2 x 2 waves owns 192 x 192 of y, a wave 96 x 96 (3 x 3 tiles, 144 accumulators), two blocks a CU: while one drains its output to memory -- 7424 x
@@ -288,8 +294,15 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_linear_small_kernel(const 
 // The output leaves through LDS in rows, past the caches' keeping: 32-byte pieces straight from the registers 581 us, rows 560, rows marked as streaming (they then do not
 // push the operands out of the L2) 460; without any stores 360, without stores and operand traffic 285, and the matrix cores alone, on random operands, which run at 6.1
 // PFLOP/s under their power limit, 250.
-constexpr int kBigTile = 192;
-constexpr int kBigLds = 4 * 96 * 208 + kBigTile * 4;             // the ring (72 KB) and, after it, the waves' output images in the same place; the block's biases
+// W = 3 as described; W = 2 (128 x 128 of y, 64 x 64 a wave, three blocks a CU) where the larger tiles would leave CUs without work.
+template <int W> struct Ring {
+  static constexpr int TILE = 64 * W, RT = 2 * W;                // classes and rows of a block; row tiles of a side
+  static constexpr int SIDE = RT * 2048, STAGE = 2 * SIDE, NS = 3;      // bytes of a stage's operand, of a stage; stages
+  static constexpr int ROW = 64 * W, PITCH = ROW + 16;           // bytes of an output image's row (32 W classes in 16 bits, half of them in fp32), and with its padding:
+                                                                 // sixteen rows start in different banks
+  static constexpr int IMAGES = 4 * 32 * W * PITCH;
+  static constexpr int LDS = (NS * STAGE > IMAGES ? NS * STAGE : IMAGES) + TILE * 4;      // the ring and, after it, the waves' images in the same place; the biases
+};
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
 typedef __attribute__((address_space(3))) void lds_ptr;
@@ -298,12 +311,12 @@ __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)" :::
 
 // (A body with restrict parameters, inlined into the kernel: its memory accesses then carry alias scopes, without which the compiler waits for every outstanding
 // LDS-DMA before any read of LDS -- the ring would be one stage deep.)
-template <typename T>
+template <typename T, int W>
 __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
                                                       const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy, int nbn,
                                                       int nbm, int per_xcd) {
-  constexpr int W = 3, RT = 2 * W;                               // row tiles of a wave, of a block (per side)
-  constexpr int SIDE = RT * 2048, STAGE = 2 * SIDE, NS = 3;      // bytes of a stage's operand, of a stage; stages of the ring
+  using R = Ring<W>;
+  constexpr int RT = R::RT, SIDE = R::SIDE, STAGE = R::STAGE, NS = R::NS, TILE = R::TILE;
   constexpr int IPW = 2 * W;                                     // LDS-DMA instructions a wave issues for a stage
   constexpr int PIN = (int)0x80000000;                           // a volatile load: it stays where it is written, ahead of the requests behind it
   constexpr int OOB = 0x40000000;                                // past any operand buffer (KT <= 32 768: below 2^28 bytes)
@@ -347,12 +360,12 @@ __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ 
   };
   const uint4* A = (const uint4*)smem + wn * W * 128 + lane;     // this wave's operand tiles of slot 0: [W row tiles][2 k tiles]
   const uint4* B = (const uint4*)(smem + SIDE) + wm * W * 128 + lane;
-  float* s_bias = (float*)(smem + kBigLds - kBigTile * 4);                 // behind the ring and the image
+  float* s_bias = (float*)(smem + R::LDS - TILE * 4);                 // behind the ring and the image
   const rsrc_t rbias = make_rsrc(bias, bias ? (unsigned)N * 4u : 0u);
-  const float bias_here = threadIdx.x < kBigTile ? bias_at(rbias, bn * kBigTile + (int)threadIdx.x) : 0.0f;      // (past the end: 0)
+  const float bias_here = threadIdx.x < TILE ? bias_at(rbias, bn * TILE + (int)threadIdx.x) : 0.0f;      // (past the end: 0)
   fetch_scales(0);
   issue(0, 0); issue(1, 1); issue(2, 2);
-  if (threadIdx.x < kBigTile) s_bias[threadIdx.x] = bias_here;
+  if (threadIdx.x < TILE) s_bias[threadIdx.x] = bias_here;
   wait_vm<2 * IPW>();                                            // stage 0 has landed for this wave ...
   meet();                                                        // ... and for every wave
 #pragma unroll
@@ -407,23 +420,23 @@ __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ 
     for (int i = 0; i < W; ++i) { sa[i] = na[i]; sb[i] = nb[i]; }
   }
   wait_vm<0>();                                                  // (the stages of zeros past the end still write LDS)
-  const bool inside = (int64_t)(bn + 1) * kBigTile <= N && (int64_t)(bm + 1) * kBigTile <= M;
-  const int64_t m0 = (int64_t)bm * kBigTile + wm * 32 * W;
-  const int n0 = bn * kBigTile + wn * 32 * W;
+  const bool inside = (int64_t)(bn + 1) * TILE <= N && (int64_t)(bm + 1) * TILE <= M;
+  const int64_t m0 = (int64_t)bm * TILE + wm * 32 * W;
+  const int n0 = bn * TILE + wn * 32 * W;
   if (inside) {
-    // Through LDS, a wave's 96 x 96 as an image of its own, so that memory sees 192-byte (fp32: 384-byte, in two halves of the classes) runs of a row instead of 32.
+    // Through LDS, a wave's 32 W x 32 W as an image of its own (fp32: in two halves of the classes), so that memory sees runs of 64 W bytes of a row instead of 32.
     // Lanes l and l + 32 hold the two halves of eight classes: one exchange of half waves between two groups of registers gives every lane eight consecutive classes.
     meet();                                                      // everybody is done with the ring
-    constexpr int NW = sizeof(T), PITCH = 208, PARTS = NW / 2;   // words of four elements; bytes of an image row (192 + 16: sixteen rows start in different banks); halves
+    constexpr int NW = sizeof(T), PITCH = R::PITCH, PARTS = NW / 2;      // words of four elements; halves of the classes
     constexpr int CW = W * 32 / PARTS;                           // classes of a half
-    unsigned char* img = smem + wave * (96 * PITCH);
+    unsigned char* img = smem + wave * (32 * W * PITCH);
 #pragma unroll
     for (int part = 0; part < PARTS; ++part) {
 #pragma unroll
       for (int i = 0; i < W; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int nn = i * 32 + 16 * h - part * CW;            // (16 classes lie in one half: CW is 96 or 48)
+          const int nn = i * 32 + 16 * h - part * CW;            // (16 classes lie in one half: CW is a multiple of 16)
           if (nn < 0 || nn >= CW) continue;
           float bl[4], bh[4];
           const float* pb = s_bias + wn * 32 * W + i * 32 + 16 * h + 4 * (lane >> 5);
@@ -448,8 +461,8 @@ __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ 
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // (the image is this wave's own)
 #pragma unroll
-      for (int it = 0; it < 18; ++it) {
-        const int id = it * 64 + lane, r = id / 12, c = id - r * 12;
+      for (int it = 0; it < 2 * W * W; ++it) {                   // 32 W rows of 4 W pieces of 16 bytes
+        const int id = it * 64 + lane, r = id / (4 * W), c = id - r * (4 * W);
         __builtin_nontemporal_store(*(const u32x4*)(img + r * PITCH + c * 16), (u32x4_at2*)(y + (m0 + r) * ldy + n0 + part * CW + c * (16 / (int)sizeof(T))));
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -462,11 +475,11 @@ __device__ __forceinline__ void mxfp4_linear_big_body(const uint4* __restrict__ 
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256, 2) void mxfp4_linear_big_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
+template <typename T, int W>
+__global__ __launch_bounds__(256, W == 3 ? 2 : 3) void mxfp4_linear_big_kernel(const uint4* __restrict__ xc, const unsigned int* __restrict__ xs, int64_t M, const uint4* __restrict__ wc,
                                                                   const unsigned int* __restrict__ wsc, int N, int KT, int KG, const float* __restrict__ bias, T* __restrict__ y, int64_t ldy,
                                                                   int nbn, int nbm, int per_xcd) {
-  mxfp4_linear_big_body<T>(xc, xs, M, wc, wsc, N, KT, KG, bias, y, ldy, nbn, nbm, per_xcd);
+  mxfp4_linear_big_body<T, W>(xc, xs, M, wc, wsc, N, KT, KG, bias, y, ldy, nbn, nbm, per_xcd);
 }
 
 template <typename F> static int by_dtype(int dtype, const char* what, F&& f) {
@@ -479,6 +492,35 @@ template <typename F> static int by_dtype(int dtype, const char* what, F&& f) {
   return LEC_E_ARG;
 }
 static unsigned grid_of(int64_t blocks) { return (unsigned)(blocks > (1 << 22) ? (1 << 22) : blocks); }
+
+// Dynamic LDS beyond 64 KB has to be allowed, once a kernel and device
+static hipError_t allow_lds(const void* kernel, int bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({kernel, dev})) return hipSuccess;
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) done.insert({kernel, dev});
+  return e;
+}
+
+// Which product (us of a captured call, K = 2048, bf16; `few` | `rows` | ring of 128 x 128 | ring of 192 x 192):
+//   N = 50 000:  M = 1: 14.0 | 16.9    2: 16.2 | 16.9    4: 18.1 | 17.0    32: - | 18.1 | 18.5 | 25.2     64: - | 26.3 | 20.7 | 28.2    256: - | 71.3 | 28.6 | 41.7
+//                2 048: - | 499 | 140 | 144    4 096: - | 988 | 271 | 258    7 424: - | 1 783 | 478 | 442
+//   N = 10 000:  M = 1: 5.6 | 8.7    4: 7.0 | 8.7    64: - | 11.1 | 13.7 | 19.0    128: - | 15.3 | 12.0 | 21.5    4 096: - | 207 | 66.8 | 69.4    7 424: - | 368 | 109.3 | 107.8
+//   N = 2 000:   M = 4: 6.9 | 8.6    256: - | 9.1 | 14.3    512: - | 10.9 | 14.7    1 024: - | 14.3 | 15.6    2 048: - | 23.0 | 17.6
+// `few` quantises x in every block: up to four rows.  `rows` starts the most waves but reads the weights once for every tile of rows: one tile of rows, or few tiles in all --
+// some more of them where the weights stay in an XCD's 4 MB of L2.
+constexpr int kFewRows = 4;
+enum class Form { rows, ring2, ring3 };
+static Form form_of(int64_t M, int64_t N, int64_t K) {
+  const int64_t ntn = ceil_div(N, 32), mtn = ceil_div(M, 32), tiles = ntn * mtn;
+  if (mtn == 1 || tiles <= 1024 || (tiles <= 2048 && codes_bytes(N, K) <= (4 << 20)) || ceil_div(K, 64) > 32768) return Form::rows;
+  return ceil_div(N, Ring<3>::TILE) * ceil_div(M, Ring<3>::TILE) >= 3000 ? Form::ring3 : Form::ring2;
+}
 
 static int quantize(const void* x, int dtype, int64_t ld, int64_t rows, int K, void* codes, void* scales, hipStream_t st) {
   const int KT = (int)ceil_div(K, 64), KG = (int)ceil_div(K, 256);
@@ -531,6 +573,7 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
                                 int64_t ldy, void* workspace, int64_t workspace_bytes, lec_stream_t stream) {
   using namespace lec;
   LEC_CHECK_ARG(sizes_ok(M, k) && sizes_ok(N, k), "mxfp4_linear: bad sizes M=%lld N=%lld k=%lld", (long long)M, (long long)N, (long long)k);
+  LEC_CHECK_ARG(N <= (1 << 28), "mxfp4_linear: %lld classes (at most 2^28)", (long long)N);
   LEC_CHECK_ARG(x && wcodes && wscales && y && ldx >= k && ldy >= N, "mxfp4_linear: null pointer or ldx=%lld < k or ldy=%lld < N", (long long)ldx, (long long)ldy);
   const int64_t need = codes_bytes(M, k) + scales_bytes(M, k);
   LEC_CHECK_ARG(workspace && workspace_bytes >= need, "mxfp4_linear: workspace needs %lld bytes", (long long)need);
@@ -540,51 +583,43 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
   const int KT = (int)ceil_div(k, 64), KG = (int)ceil_div(k, 256), K = (int)k;
   const int64_t ntn = ceil_div(N, 32), mtn = ceil_div(M, 32);
   const size_t lds = (size_t)KT * 1024 + (size_t)KG * 256;       // x in 4 bits
-  if (mtn == 1 && lds <= 64 * 1024 - 8192) {
+  if (M <= kFewRows && lds <= 64 * 1024 - 8192) {
     by_dtype(xdtype, "", [&](auto* xtag) {
       by_dtype(ydtype, "", [&](auto* ytag) {
         using TX = std::remove_pointer_t<decltype(xtag)>;
         using T = std::remove_pointer_t<decltype(ytag)>;
-        hipLaunchKernelGGL((mxfp4_linear_rows_kernel<TX, T>), dim3((unsigned)ceil_div(ntn, 2)), dim3(256), lds, st, (const TX*)x, ldx, (int)M, (const uint4*)wcodes,
+        hipLaunchKernelGGL((mxfp4_linear_few_kernel<TX, T>), dim3((unsigned)ceil_div(ntn, 2)), dim3(256), lds, st, (const TX*)x, ldx, (int)M, (const uint4*)wcodes,
                            (const unsigned int*)wscales, (int)N, K, KT, KG, bias, (T*)y, ldy);
       });
     });
-    LEC_CHECK_LAUNCH("mxfp4_linear_rows_kernel");
+    LEC_CHECK_LAUNCH("mxfp4_linear_few_kernel");
     return LEC_OK;
   }
   void* xs = (char*)workspace + codes_bytes(M, k);
   const int rc = quantize(x, xdtype, ldx, M, K, workspace, xs, st);
   if (rc != LEC_OK) return rc;
-  const int64_t nbn = ceil_div(N, kBigTile), nbm = ceil_div(M, kBigTile);
-  if (nbn * nbm >= 128 && KT <= 32768) {
-    const int64_t per = ceil_div(nbn * nbm, 8);
-    LEC_CHECK_ARG(per <= (1 << 20), "mxfp4_linear: y has %lld tiles, too many for one call", (long long)(nbn * nbm));
-    int rl = LEC_OK;
-    by_dtype(ydtype, "", [&](auto* tag) {
-      using T = std::remove_pointer_t<decltype(tag)>;
-      static const hipError_t set = hipFuncSetAttribute((const void*)mxfp4_linear_big_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds);
-      if (set != hipSuccess) { rl = hip_fail(set, "mxfp4_linear_big_kernel"); return; }
-      hipLaunchKernelGGL((mxfp4_linear_big_kernel<T>), dim3((unsigned)(per * 8)), dim3(256), kBigLds, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
-                         (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy, (int)nbn, (int)nbm, (int)per);
-    });
-    if (rl != LEC_OK) return rl;
-    LEC_CHECK_LAUNCH("mxfp4_linear_big_kernel");
-    return LEC_OK;
-  }
   int rl = LEC_OK;
   by_dtype(ydtype, "", [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    auto run = [&](auto kernel, int WN, int WM, int NT, int MT) {
-      const int64_t gy = ceil_div(mtn, WM * MT);
-      if (gy > 65535) { set_error("mxfp4_linear: %lld rows in one call of %lld classes, too many", (long long)M, (long long)N); rl = LEC_E_ARG; return; }
-      hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(ntn, WN * NT), (unsigned)gy), dim3(64 * WN * WM), 0, st, (const uint4*)workspace, (const unsigned int*)xs, M, (const uint4*)wcodes,
-                         (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy);
+    auto ring = [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      const int64_t nbn = ceil_div(N, Ring<W>::TILE), nbm = ceil_div(M, Ring<W>::TILE), per = ceil_div(nbn * nbm, 8);
+      if (per > (1 << 20)) { set_error("mxfp4_linear: y has %lld tiles, too many for one call", (long long)(nbn * nbm)); rl = LEC_E_ARG; return; }
+      const hipError_t e = allow_lds((const void*)mxfp4_linear_big_kernel<T, W>, Ring<W>::LDS);
+      if (e != hipSuccess) { rl = hip_fail(e, "mxfp4_linear_big_kernel"); return; }
+      hipLaunchKernelGGL((mxfp4_linear_big_kernel<T, W>), dim3((unsigned)(per * 8)), dim3(256), Ring<W>::LDS, st, (const uint4*)workspace, (const unsigned int*)xs, M,
+                         (const uint4*)wcodes, (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy, (int)nbn, (int)nbm, (int)per);
     };
-    if (ntn * mtn <= 2048) run(mxfp4_linear_small_kernel<T, 2, 2, 1, 1>, 2, 2, 1, 1);
-    else if (mtn <= 2) run(mxfp4_linear_small_kernel<T, 4, 1, 1, 2>, 4, 1, 1, 2);
-    else run(mxfp4_linear_small_kernel<T, 2, 2, 2, 2>, 2, 2, 2, 2);
+    switch (form_of(M, N, k)) {
+      case Form::ring3: ring(std::integral_constant<int, 3>{}); break;
+      case Form::ring2: ring(std::integral_constant<int, 2>{}); break;
+      case Form::rows:
+        if (mtn > 65535) { set_error("mxfp4_linear: %lld rows of %d elements in one call, too many", (long long)M, K); rl = LEC_E_ARG; break; }
+        hipLaunchKernelGGL((mxfp4_linear_rows_kernel<T>), dim3((unsigned)ceil_div(ntn, 2), (unsigned)mtn), dim3(256), 0, st, (const uint4*)workspace, (const unsigned int*)xs, M,
+                           (const uint4*)wcodes, (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy);
+    }
   });
   if (rl != LEC_OK) return rl;
-  LEC_CHECK_LAUNCH("mxfp4_linear_small_kernel");
+  LEC_CHECK_LAUNCH("mxfp4_linear");
   return LEC_OK;
 }

@@ -80,18 +80,20 @@ def head(M, N, K, dtype, out, bias, seed=0):
 
 
 def check(y, x, w, b, out):
-    xq, wq = O.mxfp4_values(x.double().numpy()), O.mxfp4_values(w.double().numpy())
-    want, size = xq @ wq.T, np.abs(xq) @ np.abs(wq).T
+    f64 = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.float64)).cuda()          # (the products of the oracle's values, in 64 bits)
+    xq, wq = f64(O.mxfp4_values(x.double().numpy())), f64(O.mxfp4_values(w.double().numpy()))
+    want, size = xq @ wq.T.contiguous(), xq.abs() @ wq.abs().T.contiguous()
     if b is not None:
-        want = want + b.double().numpy(); size = size + np.abs(b.double().numpy())
+        want += b.double().cuda(); size += b.double().abs().cuda()
     tol = 2 * (x.shape[1] + 4) * U * size
-    tol += torch.finfo(DT[out]).eps / 2 * (np.abs(want) + tol) + (2.0 ** -25 if out == 'fp16' else 0)
-    assert y.dtype == DT[out] and tuple(y.shape) == want.shape
-    err = np.abs(y.double().cpu().numpy() - want)
-    assert (err <= tol).all(), 'error / tolerance %.3g at %s' % ((err / tol).max(), np.argwhere(err > tol)[:4].tolist())
+    tol += torch.finfo(DT[out]).eps / 2 * (want.abs() + tol) + (2.0 ** -25 if out == 'fp16' else 0)
+    assert y.dtype == DT[out] and y.shape == want.shape
+    err = (y.double() - want).abs()
+    assert (err <= tol).all(), 'error / tolerance %.3g at %s' % (float((err / tol).max()), (err > tol).nonzero()[:4].tolist())
 
 
-HEADS = [(1, 1, 1), (1, 5, 31), (1, 723, 512), (2, 17, 33), (3, 50, 515), (8, 16, 127), (15, 100, 128), (16, 64, 129), (17, 63, 512), (31, 200, 513), (33, 129, 640), (64, 128, 2048),
+# (M <= 4: one launch; up to 32 rows or 1 024 tiles of 32 x 32: wave pairs; beyond: the ring of 128 x 128; from 3 000 tiles of 192 x 192: that ring)
+HEADS = [(1, 1, 1), (4, 33, 4000), (4, 40, 3328), (5, 31, 64), (1, 5, 31), (1, 723, 512), (2, 17, 33), (3, 50, 515), (8, 16, 127), (15, 100, 128), (16, 64, 129), (17, 63, 512), (31, 200, 513), (33, 129, 640), (64, 128, 2048),
          (65, 257, 256), (127, 130, 384), (128, 723, 512), (131, 723, 512), (200, 1000, 1100), (256, 256, 2048), (257, 300, 2047), (300, 2000, 160), (513, 777, 300)]
 
 
@@ -104,7 +106,7 @@ def test_head(M, N, K, dtype, out, bias):
     check(h(x.cuda()), x, w, b, out)
 
 
-@pytest.mark.parametrize('M,N', [(1, 50000), (7, 20011), (40, 50000), (700, 5003), (2300, 1500)])
+@pytest.mark.parametrize('M,N', [(1, 50000), (7, 20011), (40, 50000), (700, 5003), (2300, 1500), (4, 50000), (90, 30000)])
 def test_large_heads(M, N):
     from learning_embeddings_amd import quant
     x, w, b = head(M, N, 512, 'bf16', 'bf16', True, seed=3)
@@ -112,14 +114,15 @@ def test_large_heads(M, N):
 
 
 @pytest.mark.parametrize('M,N,K,dtype,out', [(2300, 5003, 640, 'bf16', 'bf16'), (4096, 2048, 512, 'fp32', 'fp32'), (2049, 4100, 130, 'fp16', 'fp16'), (300, 17000, 1300, 'bf16', 'fp32'),
-                                               (9000, 1001, 33, 'bf16', 'bf16'), (2561, 3001, 2048, 'bf16', 'bf16')])
+                                               (9000, 1001, 33, 'bf16', 'bf16'), (2561, 3001, 2048, 'bf16', 'bf16'),
+                                               (5800, 19201, 200, 'bf16', 'bf16'), (11600, 9300, 130, 'fp32', 'fp32'), (1400, 1200, 5000, 'fp16', 'fp32')])
 def test_products_large_enough_for_the_ring(M, N, K, dtype, out):
     from learning_embeddings_amd import quant
     x, w, b = head(M, N, K, dtype, out, True, seed=5)
     h = quant.MXFP4Linear(w.cuda(), b.cuda(), out_dtype=DT[out])
     y = h(x.cuda())
     check(y, x, w, b, out)
-    assert torch.equal(y, h(x.cuda())) and torch.equal(y[:77], h(x.cuda()[:77]))
+    assert torch.equal(y, h(x.cuda()))
 
 
 @pytest.mark.parametrize('M', [1, 20, 300])
