@@ -13,9 +13,7 @@
 #include "lec_common.h"
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
-#include <mutex>
-#include <set>
-#include <utility>
+#include <atomic>
 
 namespace lec {
 
@@ -493,17 +491,15 @@ template <typename F> static int by_dtype(int dtype, const char* what, F&& f) {
 }
 static unsigned grid_of(int64_t blocks) { return (unsigned)(blocks > (1 << 22) ? (1 << 22) : blocks); }
 
-// Dynamic LDS beyond 64 KB has to be allowed, once a kernel and device
-static hipError_t allow_lds(const void* kernel, int bytes) {
-  static std::mutex mu;
-  static std::set<std::pair<const void*, int>> done;
+// Dynamic LDS beyond 64 KB has to be allowed, once a kernel and device; `done` = the kernel's devices, a bit each
+static hipError_t allow_lds(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return e;
-  std::lock_guard<std::mutex> lock(mu);
-  if (done.count({kernel, dev})) return hipSuccess;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
   e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == hipSuccess) done.insert({kernel, dev});
+  if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
 
@@ -605,7 +601,8 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
       constexpr int W = decltype(w)::value;
       const int64_t nbn = ceil_div(N, Ring<W>::TILE), nbm = ceil_div(M, Ring<W>::TILE), per = ceil_div(nbn * nbm, 8);
       if (per > (1 << 20)) { set_error("mxfp4_linear: y has %lld tiles, too many for one call", (long long)(nbn * nbm)); rl = LEC_E_ARG; return; }
-      const hipError_t e = allow_lds((const void*)mxfp4_linear_big_kernel<T, W>, Ring<W>::LDS);
+      static std::atomic<unsigned long long> done{0};
+      const hipError_t e = allow_lds((const void*)mxfp4_linear_big_kernel<T, W>, Ring<W>::LDS, done);
       if (e != hipSuccess) { rl = hip_fail(e, "mxfp4_linear_big_kernel"); return; }
       hipLaunchKernelGGL((mxfp4_linear_big_kernel<T, W>), dim3((unsigned)(per * 8)), dim3(256), Ring<W>::LDS, st, (const uint4*)workspace, (const unsigned int*)xs, M,
                          (const uint4*)wcodes, (const unsigned int*)wscales, (int)N, KT, KG, bias, (T*)y, ldy, (int)nbn, (int)nbm, (int)per);

@@ -344,6 +344,9 @@ class PathLevels:
                 check(n)
             self.row_bytes[code] = n
 
+    def __reduce__(self):                                       # (copies and pickles of a criterion: by the sizes, the C array is made anew)
+        return _path_levels, (tuple(self.sizes),)
+
     @classmethod
     def of(cls, levels):
         """levels: a PathLevels, a labelmap (its `.levels`), or a sequence of sizes."""

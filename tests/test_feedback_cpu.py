@@ -85,6 +85,15 @@ def test_levels_and_settings_are_checked():
         loss.ClippedPolicyLoss(lm(), clip_low=-0.1)
 
 
+def test_criteria_can_be_copied_and_pickled():
+    import copy
+    import pickle
+    from learning_embeddings_amd import loss
+    for crit in (loss.PreferenceLoss(lm(), beta=0.3), loss.ClippedPolicyLoss(lm(), kl_coef=0.1)):
+        for c in (copy.deepcopy(crit), pickle.loads(pickle.dumps(crit))):
+            assert c.levels.sizes == [2, 3] and c.levels.L == 2 and c.levels.ptr.value
+
+
 def test_shapes_types_and_devices_are_refused():
     from learning_embeddings_amd import loss
     z, lv = torch.zeros(4, 5), [2, 3]

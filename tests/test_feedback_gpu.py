@@ -365,3 +365,48 @@ def test_captured_and_replayed(which):
         torch.cuda.synchronize()
         for i in set(((0, 1), (1, 0), (1, 1), (0, 0))[k]):
             assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+def test_a_level_of_more_runs_than_a_wave_has_lanes(dtype):
+    from learning_embeddings_amd import loss
+    lv = [5, 200001]
+    z, zd, paths, old, ref, adv = make(lv, 3, 2, dtype, seed=21, known=1.0)
+    paths[0] = [[4, 200000], [0, 0]]
+    zt = dev(z).requires_grad_()
+    lp = loss.path_log_probs(zt, dev(paths), lv)
+    want = O.path_log_probs(zd, paths, lv)
+    slack = (200001 / 2304 + 1) * U                             # the runs are more than the 24 that LT counts
+    assert (np.abs(lp.detach().cpu().numpy() - want) <= LT(lv) + slack + U * np.abs(want)).all()
+    old = (want - 0.1).astype(np.float32)
+    l, _ = loss.ClippedPolicyLoss(lv, kl_coef=0.1)(zt, dev(paths), dev(adv), dev(old), dev(ref))
+    ref[0] = want[0] + 0.1
+    l, _ = loss.ClippedPolicyLoss(lv, kl_coef=0.1)(zt, dev(paths), dev(adv), dev(old), dev(ref))
+    w_loss, _, coef = O.policy_loss(zd, paths, adv, old.astype(np.float64), ref.astype(np.float64), lv, 0.2, 0.2, 0.1, 'level')
+    q = np.abs(ref - want)
+    err = (LT(lv) + slack) * (1.3 * np.abs(adv)[:, :, None] + 0.1 * (np.exp(q) + 1)) / coef.size
+    assert abs(float(l.detach()) - w_loss) <= err.sum() + 8 * U * (np.abs(adv).max() + np.exp(q).max())
+    l.backward()
+    check_grad(zt.grad, z, zd, paths, lv, coef, err + slack * np.abs(coef) + 16 * U * np.abs(coef), dtype)
+
+
+def test_more_logits_than_31_bits_count():
+    """45 000 rows of 50 000 classes: 2.25e9 logits.  A row's result does not depend on the rows beside it, so the last rows equal the same rows alone, bit for bit."""
+    from learning_embeddings_amd import loss
+    R, C = 45000, sum(S5)
+    z = torch.empty(R, C, dtype=torch.bfloat16, device='cuda')
+    for r in range(0, R, 3000):
+        z[r:r + 3000].normal_()
+    y = torch.stack([torch.randint(0, n, (R, 2), device='cuda') for n in S5], 2)
+    ref = torch.randn(R, 2, 8, device='cuda') - 5
+    z.requires_grad_()
+    crit = loss.PreferenceLoss(S5)
+    l, rewards = crit(z, y, ref)
+    l.backward()
+    last = z.detach()[-7:].clone().requires_grad_()
+    l2, r2 = crit(last, y[-7:].contiguous(), ref[-7:].contiguous())
+    assert torch.equal(rewards[-7:], r2)
+    lp = loss.path_log_probs(z.detach(), y, S5)
+    assert torch.equal(lp[-7:], loss.path_log_probs(last.detach(), y[-7:].contiguous(), S5))
+    (l2 * (7.0 / R)).backward()                                 # 1 / P of the mean: 7 / 45 000 is not exact, so to a rounding of the coefficient and of bf16
+    assert ((z.grad[-7:].float() - last.grad.float()).abs() <= 2.0 ** -7 * last.grad.float().abs() + 1e-12).all() and last.grad.abs().max() > 0

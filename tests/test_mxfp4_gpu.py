@@ -206,3 +206,15 @@ def test_same_bits_on_another_stream_and_captured(M, N, K):
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(outs, want_k))
     assert all(torch.equal(a, c) for a, c in zip(again, want))
+
+
+def test_more_outputs_than_31_bits_count():
+    """45 000 rows x 50 000 classes: 2.25e9 outputs.  The ring sums every output's products in the same order wherever it lies: the last rows equal the same rows alone."""
+    from learning_embeddings_amd import quant
+    g = torch.Generator(device='cuda').manual_seed(0)
+    w, b = torch.randn(50000, 192, generator=g, device='cuda'), torch.randn(50000, generator=g, device='cuda')
+    x = torch.randn(45000, 192, generator=g, device='cuda').bfloat16()
+    h = quant.MXFP4Linear(w, b)
+    y = h(x)
+    assert torch.equal(y[-5000:], h(x[-5000:]))
+    check(y[-3:, -300:].contiguous(), x[-3:].cpu(), w[-300:].cpu(), b[-300:].cpu(), 'bf16')
