@@ -68,7 +68,7 @@ __device__ __forceinline__ unsigned int quantize8(const float (&v)[8], unsigned 
 
 // A block takes a row tile and a group of four k tiles (32 rows x 256 elements, one scale word a lane of the layout): half a wave reads 256 consecutive elements of a row,
 // 16 bytes a lane (32 of fp32), and the block writes its 4 KB of codes in one piece through LDS (a tile's half is padded by 8 words: the eight halves a wave writes to at
-// once start in different banks).
+// once start in different banks).  50 000 x 2 048 bf16: 54 - 63 us = 4.1 - 4.8 TB/s, and 39 us = 6.6 TB/s back (a copy: 5.1).
 template <typename T>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int K, int KT, int KG, int64_t ntask, uint4* __restrict__ codes,
                                                              unsigned int* __restrict__ scales) {
@@ -216,7 +216,7 @@ __device__ __forceinline__ bool join_halves(f32x16& acc, f32x4 (*s_half)[4][64],
   return true;
 }
 
-// A few rows: the time is the weights' way from memory, and a launch to quantise x would cost more than x is worth, so every block quantises it into LDS while its weights
+// A few rows: the time is the weights' way from memory (1 x 50 000 x 2 048: 13.4 us for 54.4 MB = 4.1 TB/s), and a launch to quantise x would cost more than x is worth, so every block quantises it into LDS while its weights
 // are under way.  x has to fit LDS beside the join: K <= 3 328.  Columns of x's tile that are no row of x are never written: a column of the product depends on its own
 // column only, and those are not stored.
 template <typename TX, typename T>
@@ -288,10 +288,12 @@ __global__ __launch_bounds__(256) void mxfp4_linear_rows_kernel(const uint4* __r
 // 50000 in bf16 are 742 MB, as long on the way as the products take -- the other one multiplies.  A stage of the ring is two k tiles (128 elements) of both operands, 24 KB;
 // three stages in LDS are filled by LDS-DMA (a wave's request is one contiguous kilobyte = one operand tile in lane order, so there is nothing to swizzle), two stages ahead.
 // Per stage a wave issues 18 MFMAs of 32 cycles and reads 12 KB of LDS: with the fills 144 KB of LDS traffic per 1152 cycles a CU, just under its 128 B / clk.
-// (256 x 256 tiles, one block a CU with 256 accumulators a wave: 638 us at that shape, 394 of them without the stores.)
-// The output leaves through LDS in rows, past the caches' keeping: 32-byte pieces straight from the registers 581 us, rows 560, rows marked as streaming (they then do not
-// push the operands out of the L2) 460; without any stores 360, without stores and operand traffic 285, and the matrix cores alone, on random operands, which run at 6.1
-// PFLOP/s under their power limit, 250.
+// The output leaves through LDS in rows, marked as streaming: it then does not push the operands out of the L2.
+// Measured, 7 424 x 50 000 x 2 048 to bf16, quantisation of x (10 us) included:  256 x 256 tiles, one block a CU, stores straight from the registers 638 us;  192 x 192, two blocks
+// a CU 581;  stores in rows 560;  marked as streaming 460;  biases from LDS 424 - 441 on four boxes = 3.5 PFLOP/s.  Without any stores 342, without stores and operand
+// traffic 285; the matrix cores alone, on random operands, run at 6.1 PFLOP/s under their power limit: 250.  Counters: matrix cores busy 52 % of the time at 1.9 GHz, 816 MB
+// written for 742 (rows of 100 000 bytes start inside cache lines), 145 MB fetched.  Deeper operand look-ahead in the body, a wave priority around the products, other
+// widths of the XCDs' bands and staggered starts of a CU's two blocks changed nothing.
 // W = 3 as described; W = 2 (128 x 128 of y, 64 x 64 a wave, three blocks a CU) where the larger tiles would leave CUs without work.
 template <int W> struct Ring {
   static constexpr int TILE = 64 * W, RT = 2 * W;                // classes and rows of a block; row tiles of a side

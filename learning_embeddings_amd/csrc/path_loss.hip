@@ -8,10 +8,17 @@
 // Both losses are functions of logp, so one pair of passes over the logits serves all three: `path_stats` (read z once) and `path_grad` (read z, write dz); between
 // them a small kernel per loss works on [R, G, L] numbers in 64 bits and leaves c.
 //
-// What bounds it: HBM, and at the small sizes the launches (2 forward, 1 backward).  A WAVE owns a run of at most 64 * NL 16-byte vectors of one level of one row,
-// all loaded before the first use, so a level of 39 078 classes spreads over 16 waves and a row of 723 over 4, with no barrier and no LDS; (max, sum) of each run
-// goes to `partials`, and whoever needs a level's lse merges its few runs again in the same order (the saved state of the backward pass IS `partials`).
-// Vectors start at the level's first class, which no alignment is promised for: the loads are 16 bytes wide at element alignment.
+// What bounds it: HBM, and at the small sizes the launches (2 forward -- 1 for the log-probabilities of a hierarchy whose levels are all one run --, 1 backward).  A WAVE owns
+// a run of at most 64 * NL 16-byte vectors of one level of one row, all loaded before the first use, so a level of 39 078 classes spreads over 16 waves and a row of 723 over 4,
+// with no barrier and no LDS; (max, sum) of each run goes to `partials`, and whoever needs a level's lse merges its few runs again in the same order (the saved state of the
+// backward pass IS `partials`).  Vectors start at the level's first class, which no alignment is promised for: the loads are 16 bytes wide at element alignment.
+// Measured (a copy of 1 GiB on the same card moves 5.1 TB/s):
+//   4 096 rows x 50 000 classes, bf16:   path_stats 85 us = 4.8 TB/s;  path_grad 160 us = 5.1 TB/s;  policy, 16 paths a row: 23 us
+//   2 048 x 50 000, fp32, two paths a row: path_stats 83 us (114 behind a pass that left 410 MB of gradient to be written back);  preference 9 us;  path_grad 71 us = 5.8 TB/s
+//     (written only: see there)
+//   256 x 723, fp32:                     4.6 | 6 | 6 us
+// Bypassing the caches with the gradient's stores moved its write-back from the next pass into this one and gained nothing; so did walking the rows backwards in one of the
+// two passes.
 #include "lec_common.h"
 #include "conv_geo.h"
 #include <hip/hip_fp16.h>
@@ -234,9 +241,10 @@ __global__ __launch_bounds__(256) void path_logp_kernel(const T* __restrict__ z,
 
 // Sum of N doubles over the grid in a fixed order; true in one thread of the last block to arrive, `total` valid there.  `counters` were zeroed by the launch before.  All
 // threads of the block call it (256 threads).  A block draws a ticket from one of 32 counters, a cache line each, and the last of each counter one from a 33rd: tickets of one
-// word are drawn one after the other, 2 048 of them in 20 us (up to 64 blocks share one).  The blocks' sums are handed over by agent-scope accesses alone, which act at the coherence point past the XCDs' L2s: a sum is
+// word are drawn one after the other (up to 64 blocks share one).  The blocks' sums are handed over by agent-scope accesses alone, which act at the coherence point past the XCDs' L2s: a sum is
 // there (vmcnt 0) before its block's ticket is drawn, and the last block asks for the sums after its own ticket has come back.  A release fence in every block would say the
-// same and write the whole L2 back each time: 2 048 blocks spent 45 of 57 us on it.
+// same and write the L2 back each time.  65 536 paths in 2 048 blocks: 57 us with the fence and one counter, 46 without the fence, 26 with 33 counters and all of the last
+// block's threads at the sums.
 constexpr unsigned int kTickets = 32;
 template <int N>
 __device__ __forceinline__ bool grid_sum(double (&v)[N] /* one value a thread */, double* __restrict__ block_sums, unsigned int* counters, double (&total)[N]) {
