@@ -98,14 +98,14 @@ template <typename T> __device__ __forceinline__ void store16(T* p, const uint4&
 __device__ __forceinline__ float fast_exp(float t) { return __builtin_amdgcn_exp2f(t * kLog2e); }
 
 // exp(x - m) for many x and one m, times a constant: one fma and one exponential an element.  x log2e - M, M = fl(m log2e), is exact but for its own rounding; what M lacks,
-// r = m log2e - M (exact in one fma), is the same for all and goes into the constant: exp(x - m) = 2^(x log2e - M) 2^-r.  Where m log2e leaves the floats' range (a level full
-// of the type's lowest value) the difference is taken first.  m = -inf (nothing finite): every term is exp(-inf) = 0.
+// r = m log2e - M (exact in one fma), is the same for all and goes into the constant: exp(x - m) = 2^(x log2e - M) 2^-r.  r is half a unit in the last place of M at most:
+// below 2^-4 for |m| < 2^20; beyond that the difference is taken first.  m = -inf (nothing finite): every term is exp(-inf) = 0.
 struct ExpAt {
   float m, M, unit;                                              // unit = 2^-r
   bool plain;
   __device__ __forceinline__ explicit ExpAt(float top) {
     m = top == -INFINITY ? 0.0f : top;
-    plain = fabsf(m) < 1e38f;                                    // (the same in all lanes: the branch below is scalar)
+    plain = fabsf(m) < 1048576.0f;                               // (the same in all lanes: the branch below is scalar)
     M = m * kLog2e;
     unit = plain ? __builtin_amdgcn_exp2f(-__builtin_fmaf(m, kLog2e, -M)) : 1.0f;
   }

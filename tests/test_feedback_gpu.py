@@ -230,6 +230,24 @@ def test_levels_full_of_the_lowest_or_highest_value_are_uniform(dtype):
     check_grad(zt.grad, z, z.double().numpy(), paths, lv, np.ones(paths.shape), np.full(paths.shape, 2 * U), dtype)
 
 
+@pytest.mark.parametrize('offset', [2.0 ** 10, 2.0 ** 19, 2.0 ** 20, 2.0 ** 24, 2.0 ** 34, 2.0 ** 60, 2.0 ** 125])
+@pytest.mark.parametrize('sign', [1, -1])
+def test_logits_far_from_zero(offset, sign):
+    """Logits a few units in the last place apart at any distance from zero: their differences are exact, and so are the softmaxes'."""
+    from learning_embeddings_amd import loss
+    lv = [4, 700, 3000]
+    rs = np.random.RandomState(3)
+    step = max(offset * 2.0 ** -23, 0.25)
+    z = torch.from_numpy((sign * offset + step * rs.randint(-8, 9, size=(5, 3704))).astype(np.float32))
+    paths = np.stack([rs.randint(0, n, size=(5, 2)) for n in lv], 2)
+    zt = dev(z).requires_grad_()
+    lp = loss.path_log_probs(zt, dev(paths), lv)
+    lp.backward(torch.ones_like(lp))
+    want = O.path_log_probs(z.double().numpy(), paths, lv)
+    assert (np.abs(lp.detach().cpu().numpy() - want) <= LT(lv) + U * np.abs(want)).all()
+    check_grad(zt.grad, z, z.double().numpy(), paths, lv, np.ones(paths.shape), np.full(paths.shape, 4 * U), 'fp32')
+
+
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
 def test_strided_transposed_and_broadcast_logits(dtype):
     from learning_embeddings_amd import loss
