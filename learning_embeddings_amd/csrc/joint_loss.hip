@@ -253,7 +253,7 @@ __device__ __forceinline__ float slot_sum(float v) {
 
 template <int T, int EPL>
 __device__ __forceinline__ void load_project(const JointParams& P, int code, bool valid, int t, Row<EPL>& r, float* stage,
-                                             const float* prefetched = nullptr) {
+                                             const float (&prefetched)[EPL], const bool have_prefetched) {      // (an array and a flag: a pointer that may be null put the array into scratch memory)
   const bool is_label = code >= 0;
   valid = valid && code_in_range(P, code);
   RowSrc src; src.f = nullptr; src.h = nullptr;
@@ -261,7 +261,7 @@ __device__ __forceinline__ void load_project(const JointParams& P, int code, boo
   const bool hyp = valid && is_label && P.label_proj == LEC_LABEL_HYP;
   const bool img = valid && (is_label ? P.label_proj == LEC_LABEL_SOFTCLIP_K : P.image_proj != LEC_IMAGE_RAW);   // soft_clip forms
   float nn;
-  if (prefetched != nullptr) {
+  if (have_prefetched) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       float v = valid ? prefetched[i] : 0.0f;                                       // (a pair this launch does not own: its row may not exist yet)
@@ -389,8 +389,8 @@ __global__ __launch_bounds__(512) void joint_loss_kernel(JointParams P_in) {
   float raw_a[EPL];
   if (pipelined) fetch_row<T, EPL>(P, code_a, t, raw_a);
   Row<EPL> U, V;
-  load_project<T, EPL>(P, ucode, task_valid && row_in_window(P, ucode), t, U, nullptr);     // every lane needs u_b, v_b: broadcast loads
-  load_project<T, EPL>(P, vcode, task_valid && row_in_window(P, vcode), t, V, nullptr);     // (an image row outside this launch's window stays zeros: it may not exist yet; no owned pair uses it -- pair_splits_windows)
+  load_project<T, EPL>(P, ucode, task_valid && row_in_window(P, ucode), t, U, nullptr, raw_a, false);     // every lane needs u_b, v_b: broadcast loads
+  load_project<T, EPL>(P, vcode, task_valid && row_in_window(P, vcode), t, V, nullptr, raw_a, false);     // (an image row outside this launch's window stays zeros: it may not exist yet; no owned pair uses it -- pair_splits_windows)
   JL_STAMP(ck1);                                      // u_b, v_b gathered and projected
   for (int it = 0; it < P.iters; ++it) {
     JL_STAMP(ci0);
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(512) void joint_loss_kernel(JointParams P_in) {
     if (pipelined) fetch_row<T, EPL>(P, code_b, t, raw_b);
     const int ocode = code_a == kNoRow ? 0 : code_a;
     Row<EPL> O;
-    load_project<T, EPL>(P, ocode, valid && q > 0, t, O, stage, pipelined ? raw_a : nullptr);
+    load_project<T, EPL>(P, ocode, valid && q > 0, t, O, stage, raw_a, pipelined);
     code_a = code_b; code_b = code_c;
     if (pipelined) {
 #pragma unroll
