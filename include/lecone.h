@@ -251,7 +251,7 @@ int lec_multilevel_ce_fwd_bwd(const float* logits, int64_t ld, const int64_t* le
  * (6b) Feedback on label paths, beside the multi-level cross-entropy: log-probabilities of paths, preference loss, clipped policy loss.
  *      No counterpart in the reference (its classifier learns from MultiLevelCELoss alone); the logits and levels are those of loss.py:29-38.
  *      logits: [R, C] of `dtype` (LEC_DTYPE_*), row stride ld >= C elements, element-aligned; level l owns level_sizes[l] consecutive columns,
- *      L <= 16, the sizes sum to C.  paths: int64 [R, G, L], G <= 64 paths a row: the class within the level, negative = not counted (its
+ *      L <= 16, the sizes sum to C <= 2^30.  paths: int64 [R, G, L], G <= 64 paths a row: the class within the level, negative = not counted (its
  *      logp is 0, its gradient 0, ref / old / coef entries there are not used); a class >= the level's size gives NaN and reads nothing.
  *      logp / ref / old / coef: fp32 [R, G, L].  Levels that no path of a row counts may hold anything (NaN included): their gradient is 0.
  *      partials: lec_path_partials_bytes() bytes written by a forward call and read by its backward.  workspace: lec_path_workspace_bytes()

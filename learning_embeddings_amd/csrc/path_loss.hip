@@ -27,6 +27,7 @@
 namespace lec {
 
 constexpr int kMaxLevels = 16;
+constexpr int kMaxClasses = 1 << 30;                             // an element's index within its level, padded to whole waves of vectors, stays within 31 bits
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct PathTable {
@@ -523,7 +524,7 @@ template <typename F> static int by_type(int dtype, F&& f) {
 
 static int table_for(PathTable& t, int dtype, int64_t R, int C, const int32_t* sizes, int L, int G) {
   LEC_CHECK_ARG(dtype == LEC_DTYPE_F32 || dtype == LEC_DTYPE_BF16 || dtype == LEC_DTYPE_F16, "path loss: unknown dtype %d", dtype);
-  LEC_CHECK_ARG(sizes && L > 0 && L <= kMaxLevels && C > 0, "path loss: bad levels L=%d (1..%d) C=%d", L, kMaxLevels, C);
+  LEC_CHECK_ARG(sizes && L > 0 && L <= kMaxLevels && C > 0 && C <= kMaxClasses, "path loss: bad levels L=%d (1..%d) C=%d (1..%d)", L, kMaxLevels, C, kMaxClasses);
   LEC_CHECK_ARG(R >= 0 && R <= (int64_t)1 << 31 && G > 0 && G <= 64, "path loss: bad sizes rows=%lld paths per row=%d (1..64)", (long long)R, G);
   return dtype == LEC_DTYPE_F32 ? build_table(t, sizes, L, C, G, Elt<float>::V, Elt<float>::NL) : build_table(t, sizes, L, C, G, Elt<_Float16>::V, Elt<_Float16>::NL);
 }

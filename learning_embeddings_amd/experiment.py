@@ -165,7 +165,8 @@ class ETHECExperiment(Experiment):
     # ---- learning from feedback on the model's answers (label paths) instead of labels; no counterpart in the reference
     def freeze_reference(self, head='mxfp4'):
         """Keeps a frozen copy of the present model as `self.reference` -- what the preference loss and the KL term measure against.  head: 'mxfp4' holds the classifier
-        in 4 bits (a quarter of bf16's weights; its log-probabilities are close to, not equal to, the model's), 'full' keeps it as it is."""
+        in 4 bits (a quarter of bf16's weights; its log-probabilities are close to, not equal to, the model's), 'full' keeps it as it is.  The copy is in
+        no checkpoint: to go on with a run, load the model it was taken from, call this, then load the run's."""
         if head not in ('mxfp4', 'full'):
             raise ValueError("head must be 'mxfp4' or 'full', got %r" % (head,))
         ref = copy.deepcopy(self.model)

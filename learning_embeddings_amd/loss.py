@@ -30,6 +30,8 @@ class MultiLevelCELoss(torch.nn.Module):
 # than on labels: on which of two paths an annotator preferred, or on a reward per sampled path.  No counterpart in the reference.
 #
 # A path is int64 [L], the class WITHIN its level as in `level_labels`, -1 (any negative) where it is not known: such an entry counts nowhere.
+#
+# A training step may be captured into a HIP graph.  As for every captured backward pass, no eager loss of the same parameters may be alive then (delete it, or keep its detach()).
 
 def path_log_probs(outputs, paths, levels):
     """Log-probabilities of label paths.  outputs [R, n_classes] (float32 / bfloat16 / float16), paths [R, L] or [R, G, L] (G paths a row), levels: a labelmap or

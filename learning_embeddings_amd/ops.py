@@ -323,7 +323,7 @@ class MultiLevelCEFn(torch.autograd.Function):
 
 # ------------------------------------------------------------------------------------------------ feedback on label paths
 DTYPE_CODE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
-MAX_PATH_LEVELS, MAX_PATHS_PER_ROW = 16, 64
+MAX_PATH_LEVELS, MAX_PATHS_PER_ROW, MAX_PATH_CLASSES = 16, 64, 1 << 30
 
 
 class PathLevels:
@@ -334,6 +334,8 @@ class PathLevels:
         if not 1 <= len(self.sizes) <= MAX_PATH_LEVELS or min(self.sizes) < 1:
             raise ValueError('levels must be 1 to %d sizes of at least one class, got %s' % (MAX_PATH_LEVELS, self.sizes))
         self.L, self.C = len(self.sizes), sum(self.sizes)
+        if self.C > MAX_PATH_CLASSES:
+            raise ValueError('at most 2^30 classes in all levels together, got %d' % self.C)
         self._arr = (C.c_int32 * self.L)(*self.sizes)
         self.ptr = C.cast(self._arr, C.c_void_p)
         self.work = int(lib.lec_path_workspace_bytes())

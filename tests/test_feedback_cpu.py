@@ -85,6 +85,21 @@ def test_levels_and_settings_are_checked():
         loss.ClippedPolicyLoss(lm(), clip_low=-0.1)
 
 
+@pytest.mark.parametrize('sizes', [[2 ** 30 + 1], [2 ** 30, 1], [2 ** 31 - 1], [2 ** 32 + 5], [3, 2 ** 32 + 5]])
+def test_hierarchies_beyond_the_kernels_indices_are_refused(sizes):
+    """2^32 + 5 is 5 in the C ABI's 32-bit sizes; a level next to 2^31 would overflow an element's index."""
+    import ctypes
+    from learning_embeddings_amd import _lib, loss, ops
+    with pytest.raises(ValueError, match='classes'):
+        ops.PathLevels.of(sizes)
+    with pytest.raises(ValueError, match='classes'):
+        loss.PreferenceLoss(sizes)
+    if sum(sizes) < 2 ** 31:
+        arr = (ctypes.c_int32 * len(sizes))(*sizes)
+        assert _lib.lib.lec_path_partials_bytes(_lib.DTYPE_F32, 1, sum(sizes), ctypes.cast(arr, ctypes.c_void_p), len(sizes)) == _lib.E_ARG
+    assert ops.PathLevels.of([2 ** 30 - 1, 1]).C == 2 ** 30
+
+
 def test_criteria_can_be_copied_and_pickled():
     import copy
     import pickle
