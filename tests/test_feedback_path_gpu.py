@@ -122,3 +122,47 @@ def test_the_4_bit_reference_is_close_to_the_full_one():
     dz = (f @ top(w).T + top(f) @ w.T) / 4 + top(f) @ top(w).T / 16
     worst = np.stack([dz[:, a:b].max(1) for a, b in O.level_slices(LEVELS)], 1)
     assert (np.abs(full - four) <= 2 * worst + 1e-5).all() and not (full == four).all()
+
+
+def test_calls_in_flight_on_two_streams_and_from_two_threads():
+    """A criterion and a head are one object each; their calls share no buffer, so calls in flight together give what they give one after the other."""
+    import threading
+    from learning_embeddings_amd import loss, quant
+    levels, R, G, K = [6, 21, 135, 561], 700, 3, 512
+    g = torch.Generator(device='cuda').manual_seed(3)
+    y = torch.stack([torch.randint(-1, n, (R, G, 1), generator=g, device='cuda') for n in levels], 3).squeeze(2)
+    adv, old = torch.randn(R, G, generator=g, device='cuda'), torch.randn(R, G, 4, generator=g, device='cuda') - 5
+    feats = [torch.randn(R, K, generator=g, device='cuda') for _ in range(8)]
+    logits = [torch.randn(R, sum(levels), generator=g, device='cuda') for _ in range(8)]
+    head = quant.MXFP4Linear(torch.randn(sum(levels), K, generator=g, device='cuda') / K ** 0.5, out_dtype=torch.float32)
+    crit = loss.ClippedPolicyLoss(levels, kl_coef=0.1)
+    def step(i):
+        ref = loss.path_log_probs(head(feats[i]), y, levels)
+        z = logits[i].detach().requires_grad_()
+        l, st = crit(z, y, adv, old, ref)
+        dz, = torch.autograd.grad(l, z)
+        return l.detach(), st, dz, ref
+    want = [step(i) for i in range(8)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None] * 8
+    for i in range(8):                                           # one thread, nothing waited for in between
+        with torch.cuda.stream(streams[i & 1]):
+            got[i] = step(i)
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for w, h in zip(want, got) for u, v in zip(w, h))
+    again, errors = [None] * 8, []
+    def work(k):
+        try:
+            with torch.cuda.stream(streams[k]):
+                for i in range(k, 8, 2):
+                    again[i] = step(i)
+        except BaseException as e:                               # (an assertion in a thread is not the test's)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors and all(torch.equal(u, v) for w, h in zip(want, again) for u, v in zip(w, h))
