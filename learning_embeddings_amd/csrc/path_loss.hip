@@ -337,13 +337,21 @@ __global__ __launch_bounds__(256) void preference_kernel(const T* __restrict__ z
 //   t = -min(rho A, clip(rho, 1 - lo, 1 + hi) A) + kl (exp(q) - q - 1),  q = ref - logp ;  dt/dlogp = -rho A [inside or on the bound] - kl expm1(q)
 // loss = sum w t.  mean over counted entries: w = 1 / N, N known only at the end of this launch -- c is left without it and `norm` = 1 / max(N, 1) multiplies it in
 // the backward pass; mean over paths: w = 1 / (entries of the path) / (R G), norm = 1.  stats = {sum w k3, sum w [clipped]}.
+// The gradient jumps where rho passes the bound, and s is a sum of 32-bit exponentials: an entry whose rho lies within 2^-20 of the bound it may cross (a sum's relative error
+// stays below (3 a + 2) 2^-24, a = the mean of m - z under the softmax) has its level summed again by the whole block in 64 bits before it is decided.  About one entry in
+// two million; the block does it for its first four (old = logp under a clip bound of 0 would ask for all of them).
 // A path is LW = the power of two >= L lanes of a wave.  The block's paths belong to a few consecutive rows: it first merges the runs of those rows' levels into LDS, as many
 // lanes to a level as there are for it (a lane that merged its own level would wait for the level of the most runs, sixteen times over for sixteen paths of a row).
 template <typename T>
-__global__ __launch_bounds__(256) void policy_kernel(const T* __restrict__ z, int64_t ld, int64_t n_paths, int LW, PathTable t, const int64_t* __restrict__ paths,
+__global__ __launch_bounds__(256, 4) void policy_kernel(const T* __restrict__ z, int64_t ld, int64_t n_paths, int LW, PathTable t, const int64_t* __restrict__ paths,
                                                      const float* __restrict__ adv, const float* __restrict__ old, const float* __restrict__ ref, float lo, float hi, float kl,
                                                      int per_path, const float2* __restrict__ partials, float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ stats,
                                                      float* __restrict__ norm, double* __restrict__ block_sums, unsigned int* counters) {
+  __shared__ unsigned long long s_near[4];
+  __shared__ double s_again[4];
+  __shared__ int64_t s_row;
+  __shared__ int s_level;
+  __shared__ double s_top;
   __shared__ double s_lse[256][2];                               // (m, log s) of the block's rows' levels: at most 256 (G = 1: one a lane; G > 1: half of that and two rows)
   const int sh = 31 - __builtin_clz(LW), l = threadIdx.x & (LW - 1), per_block = 256 >> sh;
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
@@ -386,13 +394,44 @@ __global__ __launch_bounds__(256) void policy_kernel(const T* __restrict__ z, in
     __syncthreads();
     const unsigned long long mask = __ballot(on) >> ((threadIdx.x & 63) & ~(LW - 1));
     const int cnt = __popcll(mask & ((1ull << LW) - 1ull));
+    double lp = 0.0, rho = 1.0;                         // (no old log-probabilities: on-policy, the ratio is 1)
+    bool near = false;
+    const double bound = A > 0.0 ? 1.0 + (double)hi : 1.0 - (double)lo;
+    const int k = (int)(row - row0) * t.L + l;
+    if (on) {
+      lp = ((double)zy - s_lse[k][0]) - s_lse[k][1];
+      rho = exp(lp - (old ? lo_ : lp));
+      near = old && A != 0.0 && fabs(rho - bound) < bound * 0x1p-20;
+    }
+    const unsigned long long votes = __ballot(near);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane == 0) s_near[wave] = votes;
+    __syncthreads();                                             // (but for the entries below, everybody has read s_lse, which the next round writes)
+    if (s_near[0] | s_near[1] | s_near[2] | s_near[3]) {
+      int left = 4;
+      for (int w = 0; w < 4; ++w)
+        for (unsigned long long v = s_near[w]; v && left; v &= v - 1, --left) {
+          const bool mine = wave == w && lane == __ffsll(v) - 1;
+          if (mine) { s_row = row; s_level = l; s_top = s_lse[k][0]; }
+          __syncthreads();
+          const int n = t.start[s_level + 1] - t.start[s_level];
+          const T* zl = z + s_row * ld + t.start[s_level];
+          double sum = 0.0;
+          for (int i = threadIdx.x; i < n; i += 256) sum += exp((double)Elt<T>::load(zl + i) - s_top);
+          for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+          if (lane == 0) s_again[wave] = sum;
+          __syncthreads();
+          if (mine) {
+            lp = ((double)zy - s_top) - log(s_again[0] + s_again[1] + s_again[2] + s_again[3]);
+            rho = exp(lp - lo_);
+          }
+          __syncthreads();                                       // (the next entry, or the next round, writes what was read here)
+        }
+    }
     float c = 0.0f;
     if (on) {
-      const int k = (int)(row - row0) * t.L + l;
-      const double lp = ((double)zy - s_lse[k][0]) - s_lse[k][1];
-      const double rho = exp(lp - (old ? lo_ : lp));                              // (no old log-probabilities: on-policy, the ratio is 1)
-      const bool clipped = (A > 0.0 && rho > 1.0 + (double)hi) || (A < 0.0 && rho < 1.0 - (double)lo);
-      const double gain = clipped ? (A > 0.0 ? 1.0 + (double)hi : 1.0 - (double)lo) * A : rho * A;
+      const bool clipped = (A > 0.0 && rho > bound) || (A < 0.0 && rho < bound);
+      const double gain = clipped ? bound * A : rho * A;
       double k3 = 0.0, dk = 0.0;
       if (ref) { const double d = lr_ - lp, em = expm1(d); k3 = em - d; dk = em; }
       const double w = per_path ? 1.0 / ((double)cnt * (double)n_paths) : 1.0;
@@ -403,7 +442,6 @@ __global__ __launch_bounds__(256) void policy_kernel(const T* __restrict__ z, in
       c = (float)(w * ((clipped ? 0.0 : -rho * A) - (kl != 0.0f ? (double)kl * dk : 0.0)));
     }
     if (in) coef[entry] = c;
-    __syncthreads();                                             // (the next round writes s_lse)
   }
   double total[4];
   if (grid_sum<4>(acc, block_sums, counters, total)) {

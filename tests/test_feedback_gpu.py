@@ -248,6 +248,46 @@ def test_logits_far_from_zero(offset, sign):
     check_grad(zt.grad, z, z.double().numpy(), paths, lv, np.ones(paths.shape), np.full(paths.shape, 4 * U), 'fp32')
 
 
+@pytest.mark.parametrize('name,dtype', [('ethec', 'fp32'), ('ethec', 'bf16'), ('run32', 'fp32'), ('s5', 'fp16')])
+def test_ratios_next_to_the_clip_bounds_are_decided_exactly(name, dtype):
+    """The gradient jumps at the bound, so the decision has to be the formula's own, not that of a sum with 32 bits: every 16th row has an entry whose old log-probability
+    puts log rho within half a step of a float of the bound (about 1e-7, where the error of a softmax's sum in 32 bits is as large)."""
+    from learning_embeddings_amd import loss
+    levels = LEVELS[name]
+    R = 512 if name == 'ethec' else 256
+    g = torch.Generator(device='cuda').manual_seed(21)
+    z = (torch.randn(R, sum(levels), generator=g, device='cuda') * 2.5).to(DT[dtype])
+    y = torch.stack([torch.randint(0, n, (R,), generator=g, device='cuda') for n in levels], 1)
+    exact = torch.stack([torch.log_softmax(zl.double(), 1).gather(1, yl[:, None])[:, 0] for zl, yl in zip(z.split(levels, 1), y.unbind(1))], 1)
+    adv = torch.where(torch.arange(R, device='cuda') % 32 < 16, 1.0, -1.0) * (1 + torch.rand(R, generator=g, device='cuda'))
+    hi, lo = 0.25, 0.25                                          # 1 + hi and 1 - lo are floats
+    bound = torch.where(adv > 0, 1 + hi, 1 - lo).double().log()[:, None]
+    old = (exact - bound / 2).float()                            # well inside
+    edge = torch.zeros(R, len(levels), dtype=torch.bool, device='cuda')
+    rows = torch.arange(0, R, 16, device='cuda')
+    edge[rows, rows // 16 % len(levels)] = True
+    old = torch.where(edge, (exact - bound).float(), old)
+    off = exact - old.double() - bound                           # log rho - log bound
+    hit = torch.where(adv[:, None] > 0, off > 0, off < 0) & edge
+    assert off[edge].abs().max() < 2e-6 and off[edge].abs().min() > 1e-12 and 0 < hit.sum() < edge.sum()      # near, but no ties
+    zz = z.requires_grad_()
+    l, st = loss.ClippedPolicyLoss(levels, clip_low=lo, clip_high=hi)(zz, y, adv, old)
+    grad, = torch.autograd.grad(l, zz)
+    n = R * len(levels)
+    assert round(st[1].item() * n) == hit.sum().item() and abs(st[1].item() * n - hit.sum().item()) < 1e-3
+    c = torch.where(hit, 0.0, -(exact - old.double()).exp() * adv.double()[:, None] / n)                        # d loss / d logp
+    want, s = torch.zeros_like(z, dtype=torch.float64), 0
+    for k, m in enumerate(levels):
+        p = torch.softmax(z[:, s:s + m].detach().double(), 1)
+        want[:, s:s + m] = -c[:, k:k + 1] * p
+        want[:, s:s + m].scatter_add_(1, y[:, k:k + 1], c[:, k:k + 1])
+        s += m
+    # a wrong decision moves a row's level by |c| = 0.75 / n or more; a right one by its rounding and by the 32-bit softmax's error, (3 span + 3 log(classes) + 100) 2^-24 of
+    # |c| <= 2.5 / n: with a span of 30 below 4e-5 / n (fp16's smallest step, 2^-25, is below 4e-5 / n too)
+    tol = torch.finfo(DT[dtype]).eps / 2 * want.abs() + 1e-4 / n
+    assert ((grad.double() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
 def test_strided_transposed_and_broadcast_logits(dtype):
     from learning_embeddings_amd import loss
