@@ -5,7 +5,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('LEC_LIB_PATH') or os.path.join(_HERE, 'liblecone.so')     # LEC_LIB_PATH: A/B builds of the same ABI
-ABI_VERSION = 35
+ABI_VERSION = 36
 
 OK, E_ARG, E_HIP, E_EMPTY, E_STATE = 0, -1, -2, -3, -4
 ENERGY_HYP_CONE, ENERGY_ORDER, ENERGY_EUC_CONE = 0, 1, 2
@@ -39,7 +39,7 @@ def _load():
     lib.lec_abi_version.restype = C.c_int
     if lib.lec_abi_version() != ABI_VERSION:
         raise ImportError('liblecone.so ABI %d != expected %d: rebuild' % (lib.lec_abi_version(), ABI_VERSION))
-    p, i32, i64, f32, u64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_uint64
+    p, i32, i64, f32, f64, u64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double, C.c_uint64
     sig = {
         'lec_loss_workspace_bytes': (i64, [i32, i32, i32]),
         'lec_pair_energy_fwd': (i32, [i32, p, i64, p, i64, i64, i32, f32, p, p]),
@@ -80,7 +80,7 @@ def _load():
         'lec_path_logp_fwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p]),
         'lec_path_logp_bwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p, p, p, i64, p]),
         'lec_preference_loss_fwd': (i32, [p, i32, i64, i64, i32, i32, p, i32, p, p, f32, f32, p, p, p, p, p, i64, p]),
-        'lec_policy_loss_fwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p, f32, f32, f32, i32, p, p, p, p, p, p, i64, p]),
+        'lec_policy_loss_fwd': (i32, [p, i32, i64, i64, i32, p, i32, p, i32, p, p, p, f64, f64, f32, i32, p, p, p, p, p, p, i64, p]),
         'lec_mxfp4_codes_bytes': (i64, [i64, i64]),
         'lec_mxfp4_scales_bytes': (i64, [i64, i64]),
         'lec_mxfp4_quantize': (i32, [p, i32, i64, i64, i64, p, p, p]),

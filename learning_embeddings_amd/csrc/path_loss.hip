@@ -13,7 +13,7 @@
 // with no barrier and no LDS; (max, sum) of each run goes to `partials`, and whoever needs a level's lse merges its few runs again in the same order (the saved state of the
 // backward pass IS `partials`).  Vectors start at the level's first class, which no alignment is promised for: the loads are 16 bytes wide at element alignment.
 // Measured (a copy of 1 GiB on the same card moves 5.1 TB/s):
-//   4 096 rows x 50 000 classes, bf16:   path_stats 85 us = 4.8 TB/s;  path_grad 160 us = 5.1 TB/s;  policy, 16 paths a row: 23 us
+//   4 096 rows x 50 000 classes, bf16:   path_stats 85 us = 4.8 TB/s;  path_grad 160 us = 5.1 TB/s;  policy, 16 paths a row: 24 us
 //   2 048 x 50 000, fp32, two paths a row: path_stats 83 us (114 behind a pass that left 410 MB of gradient to be written back);  preference 9 us;  path_grad 71 us = 5.8 TB/s
 //     (written only: see there)
 //   256 x 723, fp32:                     4.6 | 6 | 6 us
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256) void preference_kernel(const T* __restrict__ z
 // lanes to a level as there are for it (a lane that merged its own level would wait for the level of the most runs, sixteen times over for sixteen paths of a row).
 template <typename T>
 __global__ __launch_bounds__(256, 4) void policy_kernel(const T* __restrict__ z, int64_t ld, int64_t n_paths, int LW, PathTable t, const int64_t* __restrict__ paths,
-                                                     const float* __restrict__ adv, const float* __restrict__ old, const float* __restrict__ ref, float lo, float hi, float kl,
+                                                     const float* __restrict__ adv, const float* __restrict__ old, const float* __restrict__ ref, double lo, double hi, float kl,
                                                      int per_path, const float2* __restrict__ partials, float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ stats,
                                                      float* __restrict__ norm, double* __restrict__ block_sums, unsigned int* counters) {
   __shared__ unsigned long long s_near[4];
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(256, 4) void policy_kernel(const T* __restrict__ z,
     const int cnt = __popcll(mask & ((1ull << LW) - 1ull));
     double lp = 0.0, rho = 1.0;                         // (no old log-probabilities: on-policy, the ratio is 1)
     bool near = false;
-    const double bound = A > 0.0 ? 1.0 + (double)hi : 1.0 - (double)lo;
+    const double bound = A > 0.0 ? 1.0 + hi : 1.0 - lo;
     const int k = (int)(row - row0) * t.L + l;
     if (on) {
       lp = ((double)zy - s_lse[k][0]) - s_lse[k][1];
@@ -654,7 +654,7 @@ extern "C" int lec_preference_loss_fwd(const void* logits, int dtype, int64_t ld
 }
 
 extern "C" int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t R, int C, const int32_t* level_sizes, int L, const int64_t* paths, int G, const float* adv,
-                                   const float* old_logp, const float* ref_logp, float clip_low, float clip_high, float kl_coef, int per_path, float* loss, float* stats, float* norm, float* coef,
+                                   const float* old_logp, const float* ref_logp, double clip_low, double clip_high, float kl_coef, int per_path, float* loss, float* stats, float* norm, float* coef,
                                    void* partials, void* workspace, int64_t workspace_bytes, lec_stream_t stream) {
   using namespace lec;
   PathTable t;
@@ -662,7 +662,7 @@ extern "C" int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, in
   if (rc != LEC_OK) return rc;
   LEC_CHECK_ARG(R > 0 && logits && paths && adv && loss && stats && norm && coef && partials && ld >= C, "policy_loss: null pointer or ld=%lld < C=%d or no rows", (long long)ld, C);
   LEC_CHECK_ARG(workspace && workspace_bytes >= kWorkBytes, "policy_loss: workspace needs %lld bytes", (long long)kWorkBytes);
-  LEC_CHECK_ARG(clip_low >= 0.0f && clip_high >= 0.0f, "policy_loss: clip bounds %g, %g are negative", (double)clip_low, (double)clip_high);
+  LEC_CHECK_ARG(clip_low >= 0.0 && clip_high >= 0.0, "policy_loss: clip bounds %g, %g are negative", clip_low, clip_high);
   LEC_CHECK_ARG(kl_coef == 0.0f || ref_logp, "policy_loss: a KL coefficient needs the reference's log-probabilities");
   hipStream_t st = (hipStream_t)stream;
   unsigned int* counters = (unsigned int*)workspace;

@@ -288,6 +288,20 @@ def test_ratios_next_to_the_clip_bounds_are_decided_exactly(name, dtype):
     assert ((grad.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize('old', [-0.25, -0.18, 0.1, 0.31])
+@pytest.mark.parametrize('step', [1e-10, -1e-10])
+def test_clip_bounds_keep_64_bits(old, step):
+    """One class a level: log p is 0 exactly and rho = exp(-old).  A bound 1e-10 beyond rho does not clip, one 1e-10 short of it does; rounded to 32 bits (steps of 1e-8) it
+    would be either."""
+    from learning_embeddings_amd import loss
+    old = float(np.float32(old))
+    away = abs(np.expm1(-old)) + step
+    crit = loss.ClippedPolicyLoss([1], clip_low=away, clip_high=away)
+    z = torch.zeros(1, 1, device='cuda', requires_grad=True)
+    l, st = crit(z, torch.zeros(1, 1, dtype=torch.int64, device='cuda'), torch.tensor([1.0 if old < 0 else -1.0], device='cuda'), torch.tensor([[old]], device='cuda'))
+    assert st[1].item() == (1.0 if step < 0 else 0.0)
+
+
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
 def test_strided_transposed_and_broadcast_logits(dtype):
     from learning_embeddings_amd import loss
