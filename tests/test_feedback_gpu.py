@@ -288,6 +288,27 @@ def test_ratios_next_to_the_clip_bounds_are_decided_exactly(name, dtype):
     assert ((grad.double() - want).abs() <= tol).all()
 
 
+def test_every_ratio_at_its_bound():
+    """Bounds of 0 and the model's own log-probabilities: every ratio is 1 within a rounding, more of them next to the bound than are summed again.  Whatever is decided is
+    one of the two gradients, the loss is -mean A within the roundings, and the bits are the same every time."""
+    from learning_embeddings_amd import loss
+    z, zd, paths, _, _, adv = make(ETHEC, 300, 3, 'fp32', seed=4)
+    y, a = dev(paths), dev(adv)
+    zz = dev(z).requires_grad_()
+    old = loss.path_log_probs(zz, y, ETHEC).detach()
+    crit = loss.ClippedPolicyLoss(ETHEC, clip_low=0.0, clip_high=0.0)
+    runs = []
+    for _ in range(3):
+        l, st = crit(zz, y, a, old)
+        runs.append((l.detach(), st, torch.autograd.grad(l, zz)[0]))
+    assert all(torch.equal(u, v) for r in runs[1:] for u, v in zip(runs[0], r))
+    on = paths >= 0
+    want = -(adv[:, :, None] * on).sum() / on.sum()
+    # rho = 1 within a rounding of logp (2^-24 of at most 16) and the sum's own error (below 2^-20): 2e-6 of mean |A|; the share is a proper one
+    assert abs(runs[0][0].item() - want) <= 2e-6 * np.abs(adv).mean() + U and 0.0 <= runs[0][1][1].item() <= 1.0
+    assert torch.isfinite(runs[0][2]).all()
+
+
 @pytest.mark.parametrize('old', [-0.25, -0.18, 0.1, 0.31])
 @pytest.mark.parametrize('step', [1e-10, -1e-10])
 def test_clip_bounds_keep_64_bits(old, step):
