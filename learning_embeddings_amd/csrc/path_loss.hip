@@ -339,7 +339,8 @@ __global__ __launch_bounds__(256) void preference_kernel(const T* __restrict__ z
 // the backward pass; mean over paths: w = 1 / (entries of the path) / (R G), norm = 1.  stats = {sum w k3, sum w [clipped]}.
 // The gradient jumps where rho passes the bound, and s is a sum of 32-bit exponentials: an entry whose rho lies within 2^-20 of the bound it may cross (a sum's relative error
 // stays below (3 a + 2) 2^-24, a = the mean of m - z under the softmax) has its level summed again by the whole block in 64 bits before it is decided.  About one entry in
-// two million; the block does it for its first four (old = logp under a clip bound of 0 would ask for all of them).
+// two million.  One sum serves all entries of that level of that row -- paths that name the same class with the same old log-probability are next to the bound together --,
+// and every one of them is decided by it.
 // A path is LW = the power of two >= L lanes of a wave.  The block's paths belong to a few consecutive rows: it first merges the runs of those rows' levels into LDS, as many
 // lanes to a level as there are for it (a lane that merged its own level would wait for the level of the most runs, sixteen times over for sixteen paths of a row).
 template <typename T>
@@ -347,11 +348,8 @@ __global__ __launch_bounds__(256, 4) void policy_kernel(const T* __restrict__ z,
                                                      const float* __restrict__ adv, const float* __restrict__ old, const float* __restrict__ ref, double lo, double hi, float kl,
                                                      int per_path, const float2* __restrict__ partials, float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ stats,
                                                      float* __restrict__ norm, double* __restrict__ block_sums, unsigned int* counters) {
-  __shared__ unsigned long long s_near[4];
+  __shared__ int s_near[4];
   __shared__ double s_again[4];
-  __shared__ int64_t s_row;
-  __shared__ int s_level;
-  __shared__ double s_top;
   __shared__ double s_lse[256][2];                               // (m, log s) of the block's rows' levels: at most 256 (G = 1: one a lane; G > 1: half of that and two rows)
   const int sh = 31 - __builtin_clz(LW), l = threadIdx.x & (LW - 1), per_block = 256 >> sh;
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
@@ -403,30 +401,30 @@ __global__ __launch_bounds__(256, 4) void policy_kernel(const T* __restrict__ z,
       rho = exp(lp - (old ? lo_ : lp));
       near = old && A != 0.0 && fabs(rho - bound) < bound * 0x1p-20;
     }
-    const unsigned long long votes = __ballot(near);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (lane == 0) s_near[wave] = votes;
-    __syncthreads();                                             // (but for the entries below, everybody has read s_lse, which the next round writes)
-    if (s_near[0] | s_near[1] | s_near[2] | s_near[3]) {
-      int left = 4;
-      for (int w = 0; w < 4; ++w)
-        for (unsigned long long v = s_near[w]; v && left; v &= v - 1, --left) {
-          const bool mine = wave == w && lane == __ffsll(v) - 1;
-          if (mine) { s_row = row; s_level = l; s_top = s_lse[k][0]; }
-          __syncthreads();
-          const int n = t.start[s_level + 1] - t.start[s_level];
-          const T* zl = z + s_row * ld + t.start[s_level];
-          double sum = 0.0;
-          for (int i = threadIdx.x; i < n; i += 256) sum += exp((double)Elt<T>::load(zl + i) - s_top);
-          for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
-          if (lane == 0) s_again[wave] = sum;
-          __syncthreads();
-          if (mine) {
-            lp = ((double)zy - s_top) - log(s_again[0] + s_again[1] + s_again[2] + s_again[3]);
-            rho = exp(lp - lo_);
-          }
-          __syncthreads();                                       // (the next entry, or the next round, writes what was read here)
-        }
+    for (;;) {                                                   // the undecided entries' levels, one after the other in their order in s_lse
+      int next = 256;
+      if (__ballot(near)) {
+        next = near ? k : 256;
+        for (int w = 32; w >= 1; w >>= 1) next = min(next, __shfl_xor(next, w, 64));
+      }
+      if (lane == 0) s_near[wave] = next;
+      __syncthreads();                                           // (the last one: everybody has read s_lse, which the next round writes)
+      next = min(min(s_near[0], s_near[1]), min(s_near[2], s_near[3]));
+      if (next == 256) break;
+      const int nl = next % t.L, n = t.start[nl + 1] - t.start[nl];
+      const T* zl = z + (row0 + next / t.L) * ld + t.start[nl];
+      const double top = s_lse[next][0];
+      double sum = 0.0;
+      for (int i = threadIdx.x; i < n; i += 256) sum += exp((double)Elt<T>::load(zl + i) - top);
+      for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+      if (lane == 0) s_again[wave] = sum;
+      __syncthreads();
+      if (near && k == next) {
+        lp = ((double)zy - top) - log(s_again[0] + s_again[1] + s_again[2] + s_again[3]);
+        rho = exp(lp - lo_);
+        near = false;
+      }
     }
     float c = 0.0f;
     if (on) {
