@@ -278,7 +278,8 @@ int lec_preference_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t P
  *   t = -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1)
  *   loss[0] = mean of t;  stats[0] = mean of (exp(q) - q - 1), stats[1] = clipped share;  norm[0] = a factor of the gradient (lec_path_logp_bwd's norm)
  *   mean: per_path == 0: over the counted entries (0 when there are none); else over all R G paths of each path's mean over its counted entries.
- *   The clip bounds are 64-bit: the gradient jumps there, and next to one the kernel decides in 64 bits. */
+ *   The clip bounds are 64-bit: the gradient jumps there, and every entry so near to one that its level's 32-bit sum could
+ *   err across it is decided by that level's sum in 64 bits. */
 int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t R, int C, const int32_t* level_sizes, int L, const int64_t* paths, int G, const float* adv,
                         const float* old_logp, const float* ref_logp, double clip_low, double clip_high, float kl_coef, int per_path, float* loss, float* stats,
                         float* norm, float* coef, void* partials, void* workspace, int64_t workspace_bytes, lec_stream_t stream);

@@ -23,6 +23,8 @@
 #include "conv_geo.h"
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
+#include <algorithm>
+#include <cmath>
 
 namespace lec {
 
@@ -116,9 +118,9 @@ struct ExpAt {
 };
 
 // One run of a level of n elements at z: vectors v0 .. v0 + nv, one in 64 a lane, raw; -inf where there is none.
-template <typename T>
+template <typename T, int NL = Elt<T>::NL>
 struct Run {
-  static constexpr int V = Elt<T>::V, NL = Elt<T>::NL;
+  static constexpr int V = Elt<T>::V;
   uint4 w[NL];
   __device__ __forceinline__ void load(const T* z, int v0, int nv, int n, int lane) {
 #pragma unroll
@@ -333,21 +335,37 @@ __global__ __launch_bounds__(256) void preference_kernel(const T* __restrict__ z
   if (grid_sum<1>(acc, block_sums, counters, total)) loss[0] = (float)(total[0] / (double)P);
 }
 
+// How far, relatively, a level's 32-bit sum may be off, in units of u = 2^-24.  n classes; a lane adds up to V ceil(vectors of a run / 64) of them, the wave its lanes, `lanes`
+// lanes the runs.  A term exp(z - m): the difference, its product with log2 e and the constant, together 2.3 |z - m| over every frame it passes through, and the mean of m - z
+// under the softmax is at most log n; 2 of the exponential, 3 of ExpAt's constant.  An addition: 1 (nothing where one side is 0).  A merge of two runs: 4 (the smaller side's
+// exponential 2, its product, the addition).  4 for the products of these errors.  39 078 classes in 16 bits: 94 u.  Measured: 44 u where one class holds 92 % and 39 077 share
+// the rest, each of them losing in the same direction.
+static double sum_error(int n, int V, int vpr, int runs, int lanes) {
+  const auto halvings = [](int k) { int h = 0; while ((1 << h) < k) ++h; return h; };
+  const int adds = std::min(n, V * ((vpr + 63) / 64)) - 1 + halvings(std::min(vpr, 64)), merges = (runs + lanes - 1) / lanes - 1 + halvings(std::min(runs, lanes));
+  return (2.3 * log((double)n) + 9.0 + adds + 4.0 * merges) * 0x1p-24;
+}
+struct SumErrors { double most; float of[kMaxLevels]; };         // of a row's levels
+
 // Clipped policy loss.  Entry (r, g, l) counted: rho = exp(logp - old), A = advantage[r, g],
 //   t = -min(rho A, clip(rho, 1 - lo, 1 + hi) A) + kl (exp(q) - q - 1),  q = ref - logp ;  dt/dlogp = -rho A [inside or on the bound] - kl expm1(q)
 // loss = sum w t.  mean over counted entries: w = 1 / N, N known only at the end of this launch -- c is left without it and `norm` = 1 / max(N, 1) multiplies it in
 // the backward pass; mean over paths: w = 1 / (entries of the path) / (R G), norm = 1.  stats = {sum w k3, sum w [clipped]}.
-// The gradient jumps where rho passes the bound, and s is a sum of 32-bit exponentials: an entry whose rho lies within 2^-20 of the bound it may cross (a sum's relative error
-// stays below (3 a + 2) 2^-24, a = the mean of m - z under the softmax) has its level summed again by the whole block in 64 bits before it is decided.  About one entry in
-// two million.  One sum serves all entries of that level of that row -- paths that name the same class with the same old log-probability are next to the bound together --,
-// and every one of them is decided by it.
+// The gradient jumps where rho passes the bound, and s is a sum of 32-bit exponentials: an entry whose rho lies within what that sum may be off by (sum_error) of the bound it
+// may cross has its level summed again by the whole block in 64 bits before it is decided.  One sum serves all entries of that level of that row -- paths that name the same
+// class with the same old log-probability are next to the bound together --, and every one of them is decided by it.  One entry in 165 000 of a level of 39 078 classes where
+// log rho is spread over 0.1, and fewer of smaller levels: 14 us more for a launch that has one (4 096 rows x 16 paths x 50 000 classes, bf16).  Every entry at its bound, the
+// most there can be: 390 us instead of 110 for statistics and loss at that size, 87 instead of 12 at 512 x 8 of 723 classes.  (Told that the loop's body is rare, the compiler
+// keeps it out of the way: 0.3 us of a small launch.)
 // A path is LW = the power of two >= L lanes of a wave.  The block's paths belong to a few consecutive rows: it first merges the runs of those rows' levels into LDS, as many
 // lanes to a level as there are for it (a lane that merged its own level would wait for the level of the most runs, sixteen times over for sixteen paths of a row).
 template <typename T>
 __global__ __launch_bounds__(256, 4) void policy_kernel(const T* __restrict__ z, int64_t ld, int64_t n_paths, int LW, PathTable t, const int64_t* __restrict__ paths,
-                                                     const float* __restrict__ adv, const float* __restrict__ old, const float* __restrict__ ref, double lo, double hi, float kl,
-                                                     int per_path, const float2* __restrict__ partials, float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ stats,
+                                                     const float* __restrict__ adv, const float* __restrict__ old, const float* __restrict__ ref, SumErrors off, double lo, double hi,
+                                                     float kl, int per_path, const float2* __restrict__ partials, float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ stats,
                                                      float* __restrict__ norm, double* __restrict__ block_sums, unsigned int* counters) {
+  constexpr int V = Elt<T>::V, kAgain = 4;                       // vectors a lane asks for together when a level is summed again
+  __shared__ uint4 s_raw[256 * kAgain];                          // ... a thread's own place: the sum's loop over them is short, its 64-bit exponentials are not
   __shared__ int s_near[4];
   __shared__ double s_again[4];
   __shared__ double s_lse[256][2];                               // (m, log s) of the block's rows' levels: at most 256 (G = 1: one a lane; G > 1: half of that and two rows)
@@ -399,24 +417,38 @@ __global__ __launch_bounds__(256, 4) void policy_kernel(const T* __restrict__ z,
     if (on) {
       lp = ((double)zy - s_lse[k][0]) - s_lse[k][1];
       rho = exp(lp - (old ? lo_ : lp));
-      near = old && A != 0.0 && fabs(rho - bound) < bound * 0x1p-20;
+      near = old && A != 0.0 && fabs(rho - bound) < bound * off.most;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (;;) {                                                   // the undecided entries' levels, one after the other in their order in s_lse
       int next = 256;
-      if (__ballot(near)) {
+      if (__builtin_expect(__ballot(near) != 0, 0)) {
+        near = near && fabs(rho - bound) < bound * (double)off.of[l];
         next = near ? k : 256;
         for (int w = 32; w >= 1; w >>= 1) next = min(next, __shfl_xor(next, w, 64));
       }
       if (lane == 0) s_near[wave] = next;
       __syncthreads();                                           // (the last one: everybody has read s_lse, which the next round writes)
       next = min(min(s_near[0], s_near[1]), min(s_near[2], s_near[3]));
-      if (next == 256) break;
+      if (__builtin_expect(next == 256, 1)) break;
       const int nl = next % t.L, n = t.start[nl + 1] - t.start[nl];
       const T* zl = z + (row0 + next / t.L) * ld + t.start[nl];
       const double top = s_lse[next][0];
       double sum = 0.0;
-      for (int i = threadIdx.x; i < n; i += 256) sum += exp((double)Elt<T>::load(zl + i) - top);
+      const int nvec = (n + V - 1) / V;
+      for (int v0 = wave * 64 * kAgain; v0 < nvec; v0 += 256 * kAgain) {
+        const int nv = min(64 * kAgain, nvec - v0);
+        Run<T, kAgain> run;
+        run.load(zl, v0, nv, n, lane);
+#pragma unroll
+        for (int j = 0; j < kAgain; ++j) s_raw[j * 256 + threadIdx.x] = run.w[j];
+#pragma unroll 1
+        for (int j = 0; j * 64 < nv; ++j) {
+          const uint4 w = s_raw[j * 256 + threadIdx.x];
+#pragma unroll
+          for (int e = 0; e < V; ++e) sum += exp((double)Elt<T>::get(w, e) - top);
+        }
+      }
       for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
       if (lane == 0) s_again[wave] = sum;
       __syncthreads();
@@ -669,10 +701,18 @@ extern "C" int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, in
   int LW = 1;
   while (LW < L) LW <<= 1;
   const int64_t n = R * G, per = 256 / LW, blocks = (n + per - 1) / per;
+  const int units = (int)std::min<int64_t>((per + G - 2) / G + 1, per) * L;           // levels of the rows that a block's paths belong to, and the lanes to each (policy_kernel)
+  int lanes = 64;
+  while (lanes * units > 256) lanes >>= 1;
+  SumErrors off{};
+  for (int l = 0; l < L; ++l) {
+    const double e = sum_error(level_sizes[l], dtype == LEC_DTYPE_F32 ? Elt<float>::V : Elt<_Float16>::V, t.vpr[l], t.first[l + 1] - t.first[l], lanes);
+    off.of[l] = std::nextafter((float)e, 1.0f); off.most = std::max(off.most, (double)off.of[l]);
+  }
   by_type(dtype, [&](auto* tag) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
     hipLaunchKernelGGL((policy_kernel<T>), dim3((unsigned)(blocks > kMaxSumBlocks ? kMaxSumBlocks : blocks)), dim3(256), 0, st, (const T*)logits, ld, n, LW, t, paths, adv, old_logp,
-                       ref_logp, clip_low, clip_high, kl_coef, per_path, (const float2*)partials, coef, loss, stats, norm, (double*)((char*)workspace + kCounterBytes), counters);
+                       ref_logp, off, clip_low, clip_high, kl_coef, per_path, (const float2*)partials, coef, loss, stats, norm, (double*)((char*)workspace + kCounterBytes), counters);
   });
   LEC_CHECK_LAUNCH("policy_kernel");
   return LEC_OK;

@@ -83,6 +83,22 @@ def test_every_entry_at_its_bound_is_decided(dtype):
     assert 0.2 < check_decisions(ETHEC, z, y, adv, off_the_tie(target.float(), target), 0.0, 0.0) < 0.8
 
 
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('steps', [1.5, 20.0, 40.0, 80.0])
+@pytest.mark.parametrize('side', [1, -1])
+def test_levels_whose_sums_round_one_way(dtype, steps, side):
+    """One class at 0 and the rest together at -d: a lane that starts with 1 loses or gains up to half a step with every one of its 35 or 39 small terms, always in the same
+    direction (measured: log-probabilities off by up to 44 u for d of 11 to 13).  The ratio lies `steps` u beside its bound."""
+    R, n = 96, 39078
+    d = 11 + torch.arange(R, device='cuda') / 48 if dtype == 'fp32' else 8 + torch.arange(R, device='cuda') / 16
+    z = (-d[:, None]).expand(R, n).contiguous().to(DT[dtype])
+    z[:, 0] = 0
+    y = torch.zeros(R, 1, 1, dtype=torch.int64, device='cuda')
+    adv = torch.where(torch.arange(R, device='cuda') % 2 == 0, 1.0, -1.0)[:, None]
+    target = exact_logp(z, y, [n]) - torch.where(adv > 0, 1.25, 0.75).double().log()[:, :, None] + side * steps * U
+    check_decisions([n], z, y, adv, target.float(), 0.25, 0.25)
+
+
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
 def test_near_entries_beside_unknown_ones_and_empty_levels(dtype):
     """A row's unknown entries, rows without a known entry and levels that hold no number stay out of it."""
