@@ -105,7 +105,8 @@ def mxfp4_quantize(x):
 
 class MXFP4Linear(nn.Module):
     """y = x_4 W_4^T + b with the weights held, and x quantised on the way in, in 4 bits; sums in 32 bits, one rounding to the output's type.
-    weight [out_features, in_features], bias [out_features] or None; out_dtype None: the input's.  Frozen: see above."""
+    weight [out_features, in_features], bias [out_features] or None; out_dtype None: the input's.  Frozen: see above.
+    A state holds its sizes (`shape`) and loads into a head of the same sizes only: the buffers are padded to whole tiles and do not tell 33 x 80 from 40 x 96."""
 
     def __init__(self, weight, bias=None, out_dtype=None):
         super().__init__()
@@ -120,11 +121,22 @@ class MXFP4Linear(nn.Module):
             raise ValueError('bias must be [%d], got %s' % (self.out_features, tuple(bias.shape)))
         self.register_buffer('codes', q.codes)
         self.register_buffer('scales', q.scales)
+        self.register_buffer('shape', torch.cat([torch.full((1,), v, dtype=torch.int64, device=q.device) for v in q.shape]))
         self.register_buffer('bias', None if bias is None else bias.detach().to(device=q.device, dtype=torch.float32).contiguous().clone())
 
     @classmethod
     def from_linear(cls, linear, out_dtype=None):
         return cls(linear.weight, linear.bias, out_dtype)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        saved = state_dict.get(prefix + 'shape')
+        if saved is not None and tuple(saved.tolist()) != (self.out_features, self.in_features):
+            error_msgs.append('%s: the state is of a head of %s, this one is %d x %d' % (prefix[:-1] or 'MXFP4Linear', ' x '.join(str(v) for v in saved.tolist()), self.out_features,
+                                                                                         self.in_features))
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if saved is None and prefix + 'shape' in missing_keys and prefix + 'codes' in state_dict:       # (saved by a version that did not keep the sizes)
+            missing_keys.remove(prefix + 'shape')
 
     def extra_repr(self):
         return 'in_features=%d, out_features=%d, bias=%s, out_dtype=%s' % (self.in_features, self.out_features, self.bias is not None, self.out_dtype)

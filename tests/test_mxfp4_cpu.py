@@ -1,0 +1,51 @@
+"""The 4-bit head's host side without a GPU: states, sizes, alignment."""
+import copy
+import io
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def quant(monkeypatch):
+    """The module with a quantisation that fills its buffers with numbers that tell heads apart (the real one runs on the GPU)."""
+    from learning_embeddings_amd import quant as q
+    made = []
+
+    def numbered(w):
+        made.append(w)
+        e = lambda n: torch.full((n,), len(made), dtype=torch.uint8)
+        return q.MXFP4Tensor(e(q.codes_bytes(*w.shape)), e(q.scales_bytes(*w.shape)), w.shape)
+    monkeypatch.setattr(q, 'mxfp4_quantize', numbered)
+    return q
+
+
+@pytest.mark.parametrize('mine,other', [((33, 80), (40, 96)), ((40, 96), (33, 80)), ((33, 80), (64, 80)), ((33, 80), (33, 128)), ((5, 31), (5, 32))])
+def test_a_state_of_other_sizes_is_refused_and_changes_nothing(quant, mine, other):
+    """Both heads have the same number of 32 x 64 tiles: their buffers are of one length."""
+    a, b = quant.MXFP4Linear(torch.zeros(*mine)), quant.MXFP4Linear(torch.zeros(*other))
+    assert a.codes.shape == b.codes.shape and a.scales.shape == b.scales.shape
+    before = {k: v.clone() for k, v in a.state_dict().items()}
+    for strict in (True, False):
+        with pytest.raises(RuntimeError, match='%d x %d' % other):
+            a.load_state_dict(b.state_dict(), strict=strict)
+    with pytest.raises(RuntimeError, match='%d x %d' % other):
+        torch.nn.Sequential(a).load_state_dict(torch.nn.Sequential(b).state_dict())
+    assert all(torch.equal(v, before[k]) for k, v in a.state_dict().items())
+
+
+@pytest.mark.parametrize('bias', [False, True])
+def test_a_state_of_the_same_sizes_loads(quant, bias):
+    make = lambda: quant.MXFP4Linear(torch.zeros(33, 80), torch.randn(33) if bias else None)
+    a, b = make(), make()
+    f = io.BytesIO()
+    torch.save(b.state_dict(), f)
+    f.seek(0)
+    assert not any(a.load_state_dict(torch.load(f, weights_only=True)))
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales) and (not bias or torch.equal(a.bias, b.bias))
+    c = copy.deepcopy(b).half()
+    assert (c.out_features, c.in_features) == (33, 80) and not any(a.load_state_dict(c.state_dict()))
+    old = {k: v for k, v in make().state_dict().items() if k in ('codes', 'scales', 'bias')}        # a state without its sizes
+    assert not any(a.load_state_dict(old)) and torch.equal(a.codes, old['codes'])
+    with pytest.raises(RuntimeError, match='size mismatch'):
+        a.load_state_dict(quant.MXFP4Linear(torch.zeros(65, 80), torch.zeros(65) if bias else None).state_dict() | {'shape': torch.tensor([33, 80])})
