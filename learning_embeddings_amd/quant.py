@@ -30,10 +30,27 @@ def _matrix(x, name):
 
 
 class MXFP4Tensor:
-    """A matrix [rows, k] in 4 bits: `codes` and `scales` (uint8, in the matrix instruction's tile order -- see include/lecone.h) on one device."""
+    """A matrix [rows, k] in 4 bits: `codes` and `scales` (uint8, in the matrix instruction's tile order -- see include/lecone.h) on one device, codes_bytes(rows, k) and
+    scales_bytes(rows, k) long at least."""
 
     def __init__(self, codes, scales, shape):
         self.codes, self.scales, self.shape = codes, scales, tuple(int(v) for v in shape)
+        if len(self.shape) != 2 or min(self.shape) < 0:
+            raise ValueError('shape must be (rows, k), got %s' % (self.shape,))
+        for t, name, need in ((codes, 'codes', codes_bytes(*self.shape)), (scales, 'scales', scales_bytes(*self.shape))):
+            if t.dtype != torch.uint8:
+                raise TypeError('%s must be uint8, got %s' % (name, t.dtype))
+            if t.numel() < need or not t.is_contiguous():
+                raise ValueError('%s of a %d x %d matrix are %d contiguous bytes, got %d%s' % (name, *self.shape, need, t.numel(), '' if t.is_contiguous() else ', strided'))
+        if scales.device != codes.device:
+            raise ValueError('codes are on %s, scales on %s' % (codes.device, scales.device))
+
+    @classmethod
+    def _made(cls, codes, scales, shape):
+        """Of buffers that were made for it: nothing to check."""
+        q = cls.__new__(cls)
+        q.codes, q.scales, q.shape = codes, scales, shape
+        return q
 
     @property
     def device(self):
@@ -54,6 +71,8 @@ class MXFP4Tensor:
 
 @on_device_of(0)
 def _dequantize(codes, scales, rows, k, dtype):
+    if not codes.is_cuda:
+        dptr(codes)                                                              # raises: there is no CPU fallback
     out = torch.empty((rows, k), dtype=dtype, device=codes.device)
     check(lib.lec_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, k, out.data_ptr(), DTYPE_CODE[dtype], k, raw_stream(codes.device.index)))
     return out
@@ -99,8 +118,8 @@ def mxfp4_quantize(x):
     rows, k = z.shape
     if rows == 0:
         e = torch.empty(0, dtype=torch.uint8, device=z.device)
-        return MXFP4Tensor(e, e, (0, k))
-    return MXFP4Tensor(*_quantize(z, code, ld, rows, k), (rows, k))
+        return MXFP4Tensor._made(e, e, (0, k))
+    return MXFP4Tensor._made(*_quantize(z, code, ld, rows, k), (rows, k))
 
 
 class MXFP4Linear(nn.Module):

@@ -49,3 +49,31 @@ def test_a_state_of_the_same_sizes_loads(quant, bias):
     assert not any(a.load_state_dict(old)) and torch.equal(a.codes, old['codes'])
     with pytest.raises(RuntimeError, match='size mismatch'):
         a.load_state_dict(quant.MXFP4Linear(torch.zeros(65, 80), torch.zeros(65) if bias else None).state_dict() | {'shape': torch.tensor([33, 80])})
+
+
+def test_buffers_that_do_not_hold_the_matrix_are_refused():
+    """The kernels take codes and scales by their sizes in whole tiles: shorter buffers would be read past their end."""
+    from learning_embeddings_amd import quant
+    codes, scales = torch.zeros(4096, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    assert quant.MXFP4Tensor(codes, scales, (33, 128)).nbytes() == 4608 and quant.MXFP4Tensor(codes[:0], scales[:0], (0, 32)).dequantize().shape == (0, 32)
+    for c, s, shape in ((codes[:-1], scales, (33, 128)), (codes, scales[:-1], (33, 128)), (codes, scales, (65, 128)), (codes, scales, (33, 129)), (codes[:0], scales[:0], (1, 1)),
+                        (codes, scales[:256], (33, 1)), (codes, scales, (2 ** 31, 128))):
+        with pytest.raises(ValueError, match='bytes|too large'):
+            quant.MXFP4Tensor(c, s, shape)
+    for shape in ((33,), (33, 128, 1), (-1, 128), (33, -128)):
+        with pytest.raises(ValueError, match='shape'):
+            quant.MXFP4Tensor(codes, scales, shape)
+    with pytest.raises(TypeError, match='uint8'):
+        quant.MXFP4Tensor(codes.view(torch.int8), scales, (33, 128))
+    with pytest.raises(ValueError, match='contiguous'):
+        quant.MXFP4Tensor(torch.zeros(8192, dtype=torch.uint8)[::2], scales, (33, 128))
+    with pytest.raises(ValueError, match='on meta'):
+        quant.MXFP4Tensor(codes, scales.to('meta'), (33, 128))
+
+
+def test_buffers_in_host_memory_are_refused(quant):
+    q = quant.MXFP4Tensor(torch.zeros(1024, dtype=torch.uint8), torch.zeros(256, dtype=torch.uint8), (5, 31))
+    head = quant.MXFP4Linear(torch.zeros(5, 31))
+    for call in (q.dequantize, head.dequantize, lambda: head(torch.zeros(2, 31))):
+        with pytest.raises(RuntimeError, match='no CPU fallback'):
+            call()
