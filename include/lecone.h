@@ -290,7 +290,7 @@ int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, int64_t R, in
  *      nearest (ties to even) into {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign, saturating.  A block with a NaN or an infinity: byte 255, stands for NaN.
  *      codes:  [ceil(rows / 32)][ceil(k / 64)][64 lanes][16 bytes]: lane l holds row l % 32, elements 32 (l / 32) .. + 32 of the tile, low nibble first
  *      scales: [ceil(rows / 32)][ceil(k / 256)][64 lanes][4 bytes]: lane l's scale bytes of four consecutive 64-element tiles
- *      Padding is zero.  Both 16-byte aligned, lec_mxfp4_{codes,scales}_bytes() long (negative: bad sizes; rows <= 2^31 - 32, k <= 2^24).
+ *      Padding is zero.  Both, and the workspace, 16-byte aligned (refused otherwise); lec_mxfp4_{codes,scales}_bytes() long (negative: bad sizes; rows <= 2^31 - 32, k <= 2^24).
  *      x: [rows, k] of `dtype`, row stride ld >= k, element-aligned.  dequantize writes fp32 or bf16 (both exact).
  *      linear: y[M, N] (ydtype, ldy) = x_4 w_4^T + bias; x is quantised by the call into `workspace` (lec_mxfp4_linear_workspace_bytes, one call in flight per
  *      workspace), products are exact, sums 32-bit in a fixed order, bias (fp32 [N] or NULL) is added in 32 bits, one rounding to ydtype.

@@ -535,6 +535,7 @@ static int quantize(const void* x, int dtype, int64_t ld, int64_t rows, int K, v
 
 }  // namespace lec
 
+static bool aligned16(const void* a, const void* b) { return (((uintptr_t)a | (uintptr_t)b) & 15) == 0; }
 static bool sizes_ok(int64_t rows, int64_t k) { return rows > 0 && rows <= ((int64_t)1 << 31) - 32 && k > 0 && k <= (1 << 24); }
 
 extern "C" int64_t lec_mxfp4_codes_bytes(int64_t rows, int64_t k) { return sizes_ok(rows, k) ? lec::codes_bytes(rows, k) : LEC_E_ARG; }
@@ -544,6 +545,7 @@ extern "C" int lec_mxfp4_quantize(const void* x, int dtype, int64_t ld, int64_t 
   using namespace lec;
   LEC_CHECK_ARG(sizes_ok(rows, k), "mxfp4_quantize: bad sizes rows=%lld k=%lld", (long long)rows, (long long)k);
   LEC_CHECK_ARG(x && codes && scales && ld >= k, "mxfp4_quantize: null pointer or ld=%lld < k=%lld", (long long)ld, (long long)k);
+  LEC_CHECK_ARG(aligned16(codes, scales), "mxfp4_quantize: codes and scales have to be 16-byte aligned");
   return quantize(x, dtype, ld, rows, (int)k, codes, scales, (hipStream_t)stream);
 }
 
@@ -551,6 +553,7 @@ extern "C" int lec_mxfp4_dequantize(const void* codes, const void* scales, int64
   using namespace lec;
   LEC_CHECK_ARG(sizes_ok(rows, k), "mxfp4_dequantize: bad sizes rows=%lld k=%lld", (long long)rows, (long long)k);
   LEC_CHECK_ARG(out && codes && scales && ld >= k, "mxfp4_dequantize: null pointer or ld=%lld < k=%lld", (long long)ld, (long long)k);
+  LEC_CHECK_ARG(aligned16(codes, scales), "mxfp4_dequantize: codes and scales have to be 16-byte aligned");
   LEC_CHECK_ARG(dtype == LEC_DTYPE_F32 || dtype == LEC_DTYPE_BF16, "mxfp4_dequantize: dtype %d does not hold every value (fp32 or bf16)", dtype);
   const int KT = (int)ceil_div(k, 64), KG = (int)ceil_div(k, 256);
   const int64_t ntask = ceil_div(rows, 32) * KG;
@@ -576,6 +579,7 @@ extern "C" int lec_mxfp4_linear(const void* x, int xdtype, int64_t ldx, int64_t 
   LEC_CHECK_ARG(x && wcodes && wscales && y && ldx >= k && ldy >= N, "mxfp4_linear: null pointer or ldx=%lld < k or ldy=%lld < N", (long long)ldx, (long long)ldy);
   const int64_t need = codes_bytes(M, k) + scales_bytes(M, k);
   LEC_CHECK_ARG(workspace && workspace_bytes >= need, "mxfp4_linear: workspace needs %lld bytes", (long long)need);
+  LEC_CHECK_ARG(aligned16(wcodes, wscales) && aligned16(workspace, nullptr), "mxfp4_linear: codes, scales and workspace have to be 16-byte aligned");
   LEC_CHECK_ARG(ydtype == LEC_DTYPE_F32 || ydtype == LEC_DTYPE_BF16 || ydtype == LEC_DTYPE_F16, "mxfp4_linear: unknown dtype %d", ydtype);
   LEC_CHECK_ARG(xdtype == LEC_DTYPE_F32 || xdtype == LEC_DTYPE_BF16 || xdtype == LEC_DTYPE_F16, "mxfp4_linear: unknown dtype %d", xdtype);
   hipStream_t st = (hipStream_t)stream;

@@ -77,3 +77,16 @@ def test_buffers_in_host_memory_are_refused(quant):
     for call in (q.dequantize, head.dequantize, lambda: head(torch.zeros(2, 31))):
         with pytest.raises(RuntimeError, match='no CPU fallback'):
             call()
+
+
+@pytest.mark.parametrize('off', [1, 4, 8])
+def test_misaligned_buffers_are_refused_at_the_c_entries(off):
+    """A wave's request is a contiguous kilobyte of 16 bytes a lane.  Never dereferenced: every call is refused before its launch."""
+    import ctypes
+    from learning_embeddings_amd import _lib
+    lib, p, q = _lib.lib, ctypes.c_void_p(256), ctypes.c_void_p(256 + off)
+    for call in (lambda: lib.lec_mxfp4_quantize(p, 0, 32, 1, 32, q, p, None), lambda: lib.lec_mxfp4_quantize(p, 0, 32, 1, 32, p, q, None),
+                 lambda: lib.lec_mxfp4_dequantize(q, p, 1, 32, p, 0, 32, None), lambda: lib.lec_mxfp4_dequantize(p, q, 1, 32, p, 0, 32, None),
+                 lambda: lib.lec_mxfp4_linear(p, 0, 32, 8, q, p, 4, 32, None, p, 0, 4, p, 1 << 20, None), lambda: lib.lec_mxfp4_linear(p, 0, 32, 8, p, q, 4, 32, None, p, 0, 4, p, 1 << 20, None),
+                 lambda: lib.lec_mxfp4_linear(p, 0, 32, 8, p, p, 4, 32, None, p, 0, 4, q, 1 << 20, None)):
+        assert call() == _lib.E_ARG and b'aligned' in lib.lec_last_error()
