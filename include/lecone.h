@@ -255,7 +255,7 @@ int lec_multilevel_ce_fwd_bwd(const float* logits, int64_t ld, const int64_t* le
  *      logp is 0, its gradient 0, ref / old / coef entries there are not used); a class >= the level's size gives NaN and reads nothing.
  *      logp / ref / old / coef: fp32 [R, G, L].  Levels that no path of a row counts may hold anything (NaN included): their gradient is 0.
  *      partials: lec_path_partials_bytes() bytes written by a forward call and read by its backward.  workspace: lec_path_workspace_bytes()
- *      bytes, written from scratch by every call (nothing has to be cleared, nothing is kept); one call in flight per workspace.
+ *      bytes, written from scratch by every call (nothing has to be cleared, nothing is kept); one call in flight per workspace.  Both 8-byte aligned.
  *      Every sum has a fixed order: same inputs, same bits.  Outputs must not overlap inputs.
  * ------------------------------------------------------------------------------------------------------------- */
 #define LEC_DTYPE_F32   0

@@ -580,6 +580,8 @@ constexpr int64_t kMaxSumBlocks = 2048;
 // workspace: the arrival counters, 33 lines of 128 bytes | block sums (2048 x 4 doubles)
 constexpr int64_t kCounterBytes = 33 * 128, kWorkBytes = kCounterBytes + kMaxSumBlocks * 4 * 8;
 
+static bool aligned8(const void* a, const void* b = nullptr) { return (((uintptr_t)a | (uintptr_t)b) & 7) == 0; }       // partials: pairs of floats; workspace: atomic doubles
+
 template <typename F> static int by_type(int dtype, F&& f) {
   switch (dtype) {
     case LEC_DTYPE_F32: f((const float*)nullptr); return LEC_OK;
@@ -627,6 +629,7 @@ extern "C" int lec_path_logp_fwd(const void* logits, int dtype, int64_t ld, int6
   const int rc = table_for(t, dtype, R, C, level_sizes, L, G);
   if (rc != LEC_OK) return rc;
   LEC_CHECK_ARG(R > 0 && logits && paths && logp && partials && ld >= C, "path_logp_fwd: null pointer or ld=%lld < C=%d or no rows", (long long)ld, C);
+  LEC_CHECK_ARG(aligned8(partials), "path_logp_fwd: partials have to be 8-byte aligned");
   hipStream_t st = (hipStream_t)stream;
   const bool one_launch = t.S == t.L;                            // every level fits one wave's run: the wave that has its sum also has what its entries need
   const int rs = run_stats(logits, dtype, ld, R, t, (float2*)partials, nullptr, st, paths, one_launch ? logp : nullptr);
@@ -647,6 +650,7 @@ extern "C" int lec_path_logp_bwd(const void* logits, int dtype, int64_t ld, int6
   const int rc = table_for(t, dtype, R, C, level_sizes, L, G);
   if (rc != LEC_OK) return rc;
   LEC_CHECK_ARG(R > 0 && logits && paths && partials && coef && dlogits && ld >= C && ldg >= C, "path_logp_bwd: null pointer or ld < C or no rows");
+  LEC_CHECK_ARG(aligned8(partials), "path_logp_bwd: partials have to be 8-byte aligned");
   by_type(dtype, [&](auto* tag) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(tag)>>;
     hipLaunchKernelGGL((path_grad_kernel<T>), dim3((unsigned)wave_grid(R * t.S)), dim3(256), 0, (hipStream_t)stream, (const T*)logits, ld, R, t, paths,
@@ -666,6 +670,7 @@ extern "C" int lec_preference_loss_fwd(const void* logits, int dtype, int64_t ld
   if (rc != LEC_OK) return rc;
   LEC_CHECK_ARG(P > 0 && logits && paths && ref && loss && rewards && coef && partials && ld >= C, "preference_loss: null pointer or ld=%lld < C=%d or no pairs", (long long)ld, C);
   LEC_CHECK_ARG(workspace && workspace_bytes >= kWorkBytes, "preference_loss: workspace needs %lld bytes", (long long)kWorkBytes);
+  LEC_CHECK_ARG(aligned8(partials, workspace), "preference_loss: partials and workspace have to be 8-byte aligned");
   LEC_CHECK_ARG(label_smoothing >= 0.0f && label_smoothing <= 1.0f, "preference_loss: label_smoothing %g is not in [0, 1]", (double)label_smoothing);
   hipStream_t st = (hipStream_t)stream;
   unsigned int* counters = (unsigned int*)workspace;
@@ -692,6 +697,7 @@ extern "C" int lec_policy_loss_fwd(const void* logits, int dtype, int64_t ld, in
   if (rc != LEC_OK) return rc;
   LEC_CHECK_ARG(R > 0 && logits && paths && adv && loss && stats && norm && coef && partials && ld >= C, "policy_loss: null pointer or ld=%lld < C=%d or no rows", (long long)ld, C);
   LEC_CHECK_ARG(workspace && workspace_bytes >= kWorkBytes, "policy_loss: workspace needs %lld bytes", (long long)kWorkBytes);
+  LEC_CHECK_ARG(aligned8(partials, workspace), "policy_loss: partials and workspace have to be 8-byte aligned");
   LEC_CHECK_ARG(clip_low >= 0.0 && clip_high >= 0.0, "policy_loss: clip bounds %g, %g are negative", clip_low, clip_high);
   LEC_CHECK_ARG(kl_coef == 0.0f || ref_logp, "policy_loss: a KL coefficient needs the reference's log-probabilities");
   hipStream_t st = (hipStream_t)stream;
