@@ -290,11 +290,11 @@ __global__ __launch_bounds__(256) void mxfp4_linear_rows_kernel(const uint4* __r
 // Per stage a wave issues 18 MFMAs of 32 cycles and reads 12 KB of LDS: with the fills 144 KB of LDS traffic per 1152 cycles a CU, just under its 128 B / clk.
 // The output leaves through LDS in rows, marked as streaming: it then does not push the operands out of the L2.
 // Measured, 7 424 x 50 000 x 2 048 to bf16, quantisation of x (10 us) included:  256 x 256 tiles, one block a CU, stores straight from the registers 638 us;  192 x 192, two blocks
-// a CU 581;  stores in rows 560;  marked as streaming 460;  biases from LDS 424 - 441 on four boxes = 3.5 PFLOP/s.  Without any stores 342, without stores and operand
+// a CU 581;  stores in rows 560;  marked as streaming 460;  biases from LDS 424 - 444 on five boxes = 3.5 PFLOP/s.  Without any stores 342, without stores and operand
 // traffic 285; the matrix cores alone, on random operands, run at 6.1 PFLOP/s under their power limit: 250.  Counters: matrix cores busy 52 % of the time at 1.9 GHz, 816 MB
 // written for 742 (rows of 100 000 bytes start inside cache lines), 145 MB fetched.  Deeper operand look-ahead in the body, a wave priority around the products, other
 // widths of the XCDs' bands and staggered starts of a CU's two blocks changed nothing; one image of the block instead of one a wave gained 1 % in 16 bits and lost 1 % in fp32.
-// Blocks that stay and fetch their next tile's first stages ahead of the output were slower, 487 us where this takes 456: a later stage's arrival is counted behind the stores.
+// Blocks that stay and fetch their next tile's first stages ahead of the output were slower, in turn on one box 487 us and this 456: a later stage's arrival is counted behind the stores.
 // W = 3 as described; W = 2 (128 x 128 of y, 64 x 64 a wave, three blocks a CU) where the larger tiles would leave CUs without work.
 template <int W> struct Ring {
   static constexpr int TILE = 64 * W, RT = 2 * W;                // classes and rows of a block; row tiles of a side
@@ -511,7 +511,7 @@ static hipError_t allow_lds(const void* kernel, int bytes, std::atomic<unsigned 
 //                2 048: - | 499 | 140 | 144    4 096: - | 988 | 271 | 258    7 424: - | 1 783 | 478 | 442
 //   N = 10 000:  M = 1: 5.6 | 8.7    4: 7.0 | 8.7    64: - | 11.1 | 13.7 | 19.0    128: - | 15.3 | 12.0 | 21.5    4 096: - | 207 | 66.8 | 69.4    7 424: - | 368 | 109.3 | 107.8
 //   N = 2 000:   M = 4: 6.9 | 8.6    256: - | 9.1 | 14.3    512: - | 10.9 | 14.7    1 024: - | 14.3 | 15.6    2 048: - | 23.0 | 17.6
-// `few` quantises x in every block: up to four rows.  `rows` starts the most waves but reads the weights once for every tile of rows: one tile of rows, or few tiles in all --
+// `few` quantises x in every block: up to four rows -- at four it loses 1 us of 17 with 50 000 classes and gains 1.7 of 8.7 with 10 000 and with 2 000, which more heads have.  `rows` starts the most waves but reads the weights once for every tile of rows: one tile of rows, or few tiles in all --
 // some more of them where the weights stay in an XCD's 4 MB of L2.
 constexpr int kFewRows = 4;
 enum class Form { rows, ring2, ring3 };

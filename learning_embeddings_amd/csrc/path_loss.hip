@@ -13,9 +13,11 @@
 // with no barrier and no LDS; (max, sum) of each run goes to `partials`, and whoever needs a level's lse merges its few runs again in the same order (the saved state of the
 // backward pass IS `partials`).  Vectors start at the level's first class, which no alignment is promised for: the loads are 16 bytes wide at element alignment.
 // Measured (a copy of 1 GiB on the same card moves 5.1 TB/s):
-//   4 096 rows x 50 000 classes, bf16:   path_stats 85 us = 4.8 TB/s;  path_grad 160 us = 5.1 TB/s;  policy, 16 paths a row: 24 us
+//   4 096 rows x 50 000 classes, bf16:   path_stats 85 us = 4.8 TB/s;  path_grad 160 us = 5.1 TB/s;  policy, 16 paths a row: 25 us (40 where an entry of the
+//     largest level has to be summed again)
 //   2 048 x 50 000, fp32, two paths a row: path_stats 83 us (114 behind a pass that left 410 MB of gradient to be written back);  preference 9 us;  path_grad 71 us = 5.8 TB/s
-//     (written only: see there)
+//     (written only: see there).  A row a path, and policy with 8 paths a row: path_grad reads too, 123 us = 6.6 TB/s (the end of the statistics pass's reading is still in
+//     the caches); policy 12 us
 //   256 x 723, fp32:                     4.6 | 6 | 6 us
 // Bypassing the caches with the gradient's stores moved its write-back from the next pass into this one and gained nothing; so did walking the rows backwards in one of the
 // two passes.
