@@ -3,7 +3,7 @@ sum is.
 
 The decisions are read off twice: the clipped share times the number of entries is a whole number that has to be the right one, and an entry that is clipped contributes
 nothing to the gradient, one that is not contributes -rho A / n.  The gradient's tolerance counts u = 2^-24: (3 span + 3 log(classes) + 100) u of the sum of |coefficients|
-(span <= 30, so below 1.5e-5), and half a step of the logits' type (fp16: 2^-25 below its normal range)."""
+(span <= 30, so below 250 u), and half a step of the logits' type (fp16: 2^-25 below its normal range)."""
 import numpy as np
 import pytest
 import torch
@@ -27,8 +27,9 @@ def off_the_tie(old, target):
     return torch.where(tie(old), (target - 1e-9).float(), old)
 
 
-def check_decisions(levels, z, y, adv, old, low, high):
-    """z of the type under test, y [R, G, L], adv [R, G], old [R, G, L] fp32 -> the share of clipped entries"""
+def check_decisions(levels, z, y, adv, old, low, high, softmax_off=250):
+    """z of the type under test, y [R, G, L], adv [R, G], old [R, G, L] fp32 -> the share of clipped entries.  softmax_off: a probability's error in u (250: (3 span +
+    3 log(classes) + 100) of levels of up to 40 000 classes)"""
     from learning_embeddings_amd import loss
     exact = exact_logp(z, y, levels)
     bound = torch.where(adv > 0, 1 + high, 1 - low).double().log()[:, :, None]
@@ -49,7 +50,7 @@ def check_decisions(levels, z, y, adv, old, low, high):
         want[:, s:s + m].scatter_add_(1, y[:, :, k], c[:, :, k])
         size[:, s:s + m].scatter_add_(1, y[:, :, k], c[:, :, k].abs())
         s += m
-    tol = 1.5e-5 * size + torch.finfo(z.dtype).eps / 2 * want.abs() + (2.0 ** -25 if z.dtype == torch.float16 else 1e-37)
+    tol = softmax_off * U * size + torch.finfo(z.dtype).eps / 2 * want.abs() + (2.0 ** -25 if z.dtype == torch.float16 else 1e-37)
     bad = (grad.double() - want).abs() > tol
     assert not bad.any(), 'gradient off at %s' % bad.nonzero()[:4].tolist()
     again, st2 = loss.ClippedPolicyLoss(levels, clip_low=low, clip_high=high)(zz, y, adv, old)
@@ -57,10 +58,12 @@ def check_decisions(levels, z, y, adv, old, low, high):
     return hit.double().mean().item()
 
 
-@pytest.mark.parametrize('levels,R,G', [(ETHEC, 256, 16), (ETHEC, 50, 64), (S5, 24, 16), ([2, 3], 333, 5), ([3], 7, 2), (list(range(2, 18)), 40, 9)])
+@pytest.mark.parametrize('levels,R,G', [(ETHEC, 256, 16), (ETHEC, 50, 64), (S5, 24, 16), ([2, 3], 333, 5), ([3], 7, 2), (list(range(2, 18)), 40, 9), (list(range(2, 18)), 333, 1),
+                                           (ETHEC, 9000, 16), ([2], 70000, 8)])
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
 def test_paths_that_share_a_class_are_decided_alike(levels, R, G, dtype):
-    """All paths of a row name the same classes with the same log-probabilities of the sampler, every one of them next to its bound: many entries of few levels."""
+    """All paths of a row name the same classes with the same log-probabilities of the sampler, every one of them next to its bound: many entries of few levels.
+    (The last two: more paths than the grid's blocks take in one round.)"""
     g = torch.Generator(device='cuda').manual_seed(5)
     z = (torch.randn(R, sum(levels), generator=g, device='cuda') * 2.5).to(DT[dtype])
     y = torch.stack([torch.randint(0, n, (R, 1), generator=g, device='cuda') for n in levels], 2).expand(R, G, len(levels)).contiguous()
@@ -97,6 +100,19 @@ def test_levels_whose_sums_round_one_way(dtype, steps, side):
     adv = torch.where(torch.arange(R, device='cuda') % 2 == 0, 1.0, -1.0)[:, None]
     target = exact_logp(z, y, [n]) - torch.where(adv > 0, 1.25, 0.75).double().log()[:, :, None] + side * steps * U
     check_decisions([n], z, y, adv, target.float(), 0.25, 0.25)
+
+
+@pytest.mark.parametrize('steps', [20.0, 100.0, 300.0])
+@pytest.mark.parametrize('side', [1, -1])
+def test_a_level_of_a_million_classes(steps, side):
+    """456 runs, merged one after the other by a single lane: its sum was measured 152 u off."""
+    R, n = 32, 1 << 20
+    z = -(11 + torch.arange(R, device='cuda') / 16)[:, None].expand(R, n).contiguous()
+    z[:, 0] = 0
+    y = torch.zeros(R, 1, 1, dtype=torch.int64, device='cuda')
+    adv = torch.where(torch.arange(R, device='cuda') % 2 == 0, 1.0, -1.0)[:, None]
+    target = exact_logp(z, y, [n]) - torch.where(adv > 0, 1.25, 0.75).double().log()[:, :, None] + side * steps * U
+    check_decisions([n], z, y, adv, target.float(), 0.25, 0.25, softmax_off=2000)
 
 
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
