@@ -290,11 +290,11 @@ __global__ __launch_bounds__(256) void mxfp4_linear_rows_kernel(const uint4* __r
 // Per stage a wave issues 18 MFMAs of 32 cycles and reads 12 KB of LDS: with the fills 144 KB of LDS traffic per 1152 cycles a CU, just under its 128 B / clk.
 // The output leaves through LDS in rows, marked as streaming: it then does not push the operands out of the L2.
 // Measured, 7 424 x 50 000 x 2 048 to bf16, quantisation of x (10 us) included:  256 x 256 tiles, one block a CU, stores straight from the registers 638 us;  192 x 192, two blocks
-// a CU 581;  stores in rows 560;  marked as streaming 460;  biases from LDS 424 - 444 on five boxes = 3.5 PFLOP/s.  Without any stores 342, without stores and operand
+// a CU 581;  stores in rows 560;  marked as streaming 460;  biases from LDS 424 - 444 on five machines = 3.5 PFLOP/s.  Without any stores 342, without stores and operand
 // traffic 285; the matrix cores alone, on random operands, run at 6.1 PFLOP/s under their power limit: 250.  Counters: matrix cores busy 52 % of the time at 1.9 GHz, 816 MB
 // written for 742 (rows of 100 000 bytes start inside cache lines), 145 MB fetched.  Deeper operand look-ahead in the body, a wave priority around the products, other
 // widths of the XCDs' bands and staggered starts of a CU's two blocks changed nothing; one image of the block instead of one a wave gained 1 % in 16 bits and lost 1 % in fp32.
-// Blocks that stay and fetch their next tile's first stages ahead of the output were slower, in turn on one box 487 us and this 456: a later stage's arrival is counted behind the stores.
+// Blocks that stay and fetch their next tile's first stages ahead of the output were slower, in turn on one machine 487 us and this 456: a later stage's arrival is counted behind the stores.
 // W = 3 as described; W = 2 (128 x 128 of y, 64 x 64 a wave, three blocks a CU) where the larger tiles would leave CUs without work.
 template <int W> struct Ring {
   static constexpr int TILE = 64 * W, RT = 2 * W;                // classes and rows of a block; row tiles of a side
